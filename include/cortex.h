@@ -217,7 +217,8 @@ CORTEX_API int cortex_seq_rewind(void *state, const int *slots, int n, int pos);
  * on the state's stream and its algorithmic bytes and FLOPs are counted.
  * kind: 0 embedding+norm, 1 rmsnorm, 2 QKV projection, 3 attention,
  * 4 Wo projection, 5 W_up, 6 W_down, 7 logits projection, 8 sampler,
- * 9 the persistent kernel of a whole one- or two-row fp32 decode pass.
+ * 9 the persistent kernel of a whole one- or two-row fp32 decode pass,
+ * 10 the scores of cortex_score_batch.
  * Enabling (or disabling) clears the counters; reading waits for the
  * stream. */
 CORTEX_API int cortex_profile_enable(void *state, int on);
@@ -370,6 +371,104 @@ CORTEX_API void cortex_extract_grad_layer(void *state, int layer_idx, int tensor
  * cortex_train_apply: its factor, the gradient norm and whether it applied.
  * Returns 0, or -1 before the first update. */
 CORTEX_API int cortex_train_info(void *state, int *adam_steps, float *clip_factor, float *grad_norm, int *clipped);
+
+/* ------------------------------------------------------------------------ */
+/* What the model says about given tokens, and learning from another model.  */
+/* No counterpart in the reference.  Three stateless calls over rows of      */
+/* vocabulary logits in device memory (beside cortex_sample), then the same  */
+/* on a state's own passes and training step.                                */
+/*                                                                           */
+/* logits[rows][ld] (row stride ld >= vocab, vocab <= 524288) are fp32, bf16 */
+/* or fp16; any alignment of the rows to an element is taken, 16-byte        */
+/* aligned rows are fastest.  p = softmax(logits / temperature) of a row,    */
+/* 0.001 <= temperature <= 1000.  Statistics are held in fp32 or more.       */
+/*  - An id outside [0, vocab) is padding: log probability 0, no teacher     */
+/*    mass, no gradient.                                                     */
+/*  - A logit of -inf is masked: p = 0, log p = -inf, gradient 0.  A row     */
+/*    masked everywhere has entropy 0.                                       */
+/*  - A row holding a NaN or +inf has no distribution: its results are NaN,  */
+/*    its alternatives' ids -1.                                              */
+/* Work is queued on `stream` (a cudaStream_t of the device that holds the   */
+/* arrays; NULL = its legacy default stream), whichever device is current;   */
+/* nothing is allocated and no workspace is shared, so calls may overlap and */
+/* be captured into CUDA graphs.  Results do not depend on the other rows of */
+/* a call, and repeat bit for bit.                                           */
+/* ------------------------------------------------------------------------ */
+
+#define SNAI_DTYPE_FP32 0
+#define SNAI_DTYPE_BF16 1
+#define SNAI_DTYPE_FP16 2
+
+/* Scores of each row: logprob[rows][n_tok] = log p of tokens[rows][n_tok]
+ * (0 <= n_tok <= 512; both may be NULL when n_tok is 0), entropy[rows] in
+ * nats (or NULL), and the top_k alternatives (0 <= top_k <= min(512, vocab))
+ * top_ids[rows][top_k] in descending order of logit, equal logits in
+ * ascending order of id, with top_logprob[rows][top_k] = their log p. */
+CORTEX_API int cortex_score(const void *logits, int dtype, int rows, int vocab, long long ld, const int *tokens,
+                            int n_tok, double temperature, int top_k, float *logprob, float *entropy, int *top_ids,
+                            float *top_logprob, void *stream);
+
+/* The gradient of cortex_score with respect to the logits:
+ *   grad = d/dlogits [ sum g_logprob[r][j] * logprob[r][j] + sum g_entropy[r] * entropy[r] ],
+ * g_logprob[rows][n_tok] (a token listed twice counts twice), g_entropy[rows]
+ * or NULL.  grad[rows][grad_ld] has the logits' type, rounded once; it may be
+ * the logits' own memory (same pointer and stride), else it must share no
+ * element with them.  Columns past vocab are left as they are.  A row whose
+ * tokens are all padding and whose g_entropy is 0 gets zeros, whatever its
+ * logits hold.  To propagate through alternatives, list them as tokens. */
+CORTEX_API int cortex_score_grad(const void *logits, int dtype, int rows, int vocab, long long ld, const int *tokens,
+                                 int n_tok, double temperature, const float *g_logprob, const float *g_entropy,
+                                 void *grad, long long grad_ld, void *stream);
+
+/* Distillation from a teacher's top logits.  Per row, over the listed
+ * teacher_ids[rows][top_k] / teacher_logits[rows][top_k] (1 <= top_k <= 512;
+ * shorter lists are padded with ids of -1, an id listed twice counts twice):
+ *   loss = (1 - label_weight) * temperature^2 * KL(q || p)
+ *          + label_weight * -log softmax(logits)[labels[r]]     (no temperature)
+ * rest 0: q = softmax(teacher_logits / temperature) over the list, 0 elsewhere.
+ * rest 1: teacher_logits are the teacher's log probabilities at this
+ *   temperature already (cortex_score's top_logprob): q = exp(teacher_logits),
+ *   and what the list leaves of 1 (at least 0) is one more outcome, set
+ *   against the student's probability of all unlisted ids.  Where the student
+ *   has none (every unlisted id masked) that outcome is left out.
+ * A row whose list and label are all padding has loss 0 and gradient 0,
+ * whatever its logits hold. */
+typedef struct snai_distill_params {
+  double temperature;
+  double label_weight; /* 0 <= label_weight <= 1; above 0 needs labels */
+  int rest;
+} snai_distill_params;
+
+/* loss[rows]; grad (or NULL: the loss alone) = row_grad[r] (1 when NULL) *
+ * dloss[r]/dlogits, stored as cortex_score_grad's.  One call reads the logits
+ * once for both, so a training step makes no separate backward call. */
+CORTEX_API int cortex_distill(const void *logits, int dtype, int rows, int vocab, long long ld,
+                              const int *teacher_ids, const float *teacher_logits, int top_k, const int *labels,
+                              const float *row_grad, const snai_distill_params *params, float *loss, void *grad,
+                              long long grad_ld, void *stream);
+
+/* Feeds tokens[batch][n_tok] as cortex_forward_batch does and scores every
+ * position: after token i of slot b, logprob[b][i] is the log probability of
+ * targets[b][i] (NULL targets and logprob: none), entropy[b][i] the entropy
+ * (or NULL) and top_ids / top_logprob[b][i][top_k] the alternatives (top_k 0:
+ * none), as cortex_score gives them for that position's logits.  Entries of
+ * positions past ctx are left as they are.  The logits of each slot's last
+ * token stay for cortex_decode_batch.  flags: SNAI_HOST_PTRS or
+ * SNAI_DEVICE_PTRS (all arrays but slots).  The logits of up to 1024
+ * positions at a time live in a buffer made by the state's first call. */
+CORTEX_API int cortex_score_batch(void *state, const int *tokens, int batch, int n_tok, const int *slots,
+                                  const int *targets, double temperature, int top_k, float *logprob, float *entropy,
+                                  int *top_ids, float *top_logprob, int flags);
+
+/* cortex_train_grads with cortex_distill's loss in place of the reference's
+ * cross-entropy (core/cortex.nim:604-616): forward and backward over act =
+ * min(num_tokens, ctx) input ids against teacher_ids / teacher_logits
+ * [num_tokens][top_k] and, with label_weight above 0, labels[num_tokens] (host
+ * arrays; padding as above).  The gradients of the summed loss are left for
+ * cortex_train_apply; *loss is the mean over the act positions. */
+CORTEX_API int cortex_distill_grads(void *state, const int *raw_inputs, const int *teacher_ids,
+                                    const float *teacher_logits, int top_k, const int *labels, int num_tokens,
+                                    const snai_distill_params *params, float *loss);
 
 /* Number of kernels the state has launched since it was created. */
 CORTEX_API long long cortex_kernel_launches(void *state);

@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(HERE, "libcortex.so")
 
 PREC_FP32, PREC_TF32, PREC_BF16 = 0, 1, 2
 HOST_PTRS, DEVICE_PTRS = 0, 1
+DTYPE_FP32, DTYPE_BF16, DTYPE_FP16 = 0, 1, 2
 
 c_int, c_float, c_double, c_void_p, c_char_p = (ctypes.c_int, ctypes.c_float, ctypes.c_double,
                                                 ctypes.c_void_p, ctypes.c_char_p)
@@ -31,6 +32,12 @@ class SampleParams(ctypes.Structure):
         ("top_p", c_double),
         ("nan_guard", c_int),
     ]
+
+
+class DistillParams(ctypes.Structure):
+    """snai_distill_params: the constants of a distillation loss."""
+
+    _fields_ = [("temperature", c_double), ("label_weight", c_double), ("rest", c_int)]
 
 
 # name -> (restype, argtypes); the full export list of include/cortex.h
@@ -98,6 +105,17 @@ SIGNATURES = {
     "cortex_extract_grad_layer": (None, [c_void_p, c_int, c_int, c_void_p, c_int]),
     "cortex_train_info": (c_int, [c_void_p, ctypes.POINTER(c_int), ctypes.POINTER(c_float), ctypes.POINTER(c_float),
                                   ctypes.POINTER(c_int)]),
+    "cortex_score": (c_int, [c_void_p, c_int, c_int, c_int, ctypes.c_longlong, c_void_p, c_int, c_double, c_int,
+                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "cortex_score_grad": (c_int, [c_void_p, c_int, c_int, c_int, ctypes.c_longlong, c_void_p, c_int, c_double,
+                                  c_void_p, c_void_p, c_void_p, ctypes.c_longlong, c_void_p]),
+    "cortex_distill": (c_int, [c_void_p, c_int, c_int, c_int, ctypes.c_longlong, c_void_p, c_void_p, c_int, c_void_p,
+                               c_void_p, ctypes.POINTER(DistillParams), c_void_p, c_void_p, ctypes.c_longlong,
+                               c_void_p]),
+    "cortex_score_batch": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_double, c_int, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_int]),
+    "cortex_distill_grads": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                     ctypes.POINTER(DistillParams), ctypes.POINTER(c_float)]),
 }
 
 _lib = None

@@ -46,17 +46,6 @@ int env_int(const char *name, int def) {
   return atoi(v);
 }
 
-struct DeviceGuard {
-  int prev = -1, want;
-  explicit DeviceGuard(int d) : want(d) {
-    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev != d) cudaSetDevice(d);
-  }
-  ~DeviceGuard() {
-    if (prev >= 0 && prev != want) cudaSetDevice(prev);
-  }
-};
-
 size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // Carves aligned sub-buffers out of one allocation.
@@ -124,6 +113,7 @@ void free_engine(Engine *e) {
   cudaFree(e->unif_all);
   cudaFree(e->ids_all);
   cudaFree(e->avg_tmp);
+  cudaFree(e->score_buf);
   train_free(*e);
   if (e->own_stream) cudaStreamDestroy(e->own_stream);
   delete e;
@@ -747,6 +737,39 @@ extern "C" int cortex_train_grads(void *state, const int *raw_inputs, const int 
   return rc ? rc : check_device_error(e);
 }
 
+extern "C" int cortex_distill_grads(void *state, const int *raw_inputs, const int *teacher_ids,
+                                    const float *teacher_logits, int top_k, const int *labels, int num_tokens,
+                                    const snai_distill_params *params, float *loss) {
+  clear_error();
+  if (!state || !params || !loss) {
+    set_error("cortex_distill_grads: NULL state, params or loss");
+    return -1;
+  }
+  Engine &e = *static_cast<Engine *>(state);
+  const int act = std::min(num_tokens, e.d.ctx);
+  *loss = 0.0f;
+  DistillLaunch s;
+  s.V = e.d.V;
+  s.ld = e.d.V;
+  s.teacher_ids = teacher_ids;
+  s.teacher_logits = teacher_logits;
+  s.top_k = top_k;
+  s.labels = labels;
+  s.temperature = params->temperature;
+  s.label_weight = params->label_weight;
+  s.rest = params->rest;
+  const int bad = check_distill("cortex_distill_grads", s);
+  if (bad) return bad;
+  if (act <= 0) return 0;
+  if (!raw_inputs || !teacher_ids || !teacher_logits || (params->label_weight > 0.0 && !labels)) {
+    set_error("cortex_distill_grads: NULL token, teacher or label arrays");
+    return -1;
+  }
+  DeviceGuard g(e.device);
+  const int rc = train_grads(e, raw_inputs, labels, act, loss, &s);
+  return rc ? rc : check_device_error(e);
+}
+
 extern "C" int cortex_train_apply(void *state, float lr, float scale) {
   clear_error();
   if (!state) {
@@ -871,6 +894,152 @@ extern "C" int cortex_forward_batch(void *state, const int *tokens, int batch, i
     return -1;
   }
   return forward_batch(*static_cast<Engine *>(state), tokens, batch, n_tok, slots, logits, flags);
+}
+
+// Positions scored at a time: their logits fill at most 256 MB.
+static int score_rows_max(const Engine &e) {
+  const size_t fit = (size_t(256) << 20) / (sizeof(float) * (size_t)e.d.V);
+  return std::min({e.m_max, 1024, (int)std::max<size_t>(fit, 16)});
+}
+
+// Logits, targets and scores of score_rows_max positions, made once.
+static int score_buffers(Engine &e) {
+  if (e.score_buf) return 0;
+  const size_t R = score_rows_max(e);
+  Carver c;
+  c.add(&e.score_logits, R * e.d.V);
+  c.add(&e.score_tok, R);
+  c.add(&e.score_lp, R);
+  c.add(&e.score_ent, R);
+  c.add(&e.score_ids, R * kScoreMaxK);
+  c.add(&e.score_top, R * kScoreMaxK);
+  if (cudaMalloc(&e.score_buf, c.off) != cudaSuccess) {
+    cudaGetLastError();
+    e.score_buf = nullptr;
+    set_error("device allocation of the scored positions' logits failed (%zu B)", c.off);
+    return -3;
+  }
+  c.place(e.score_buf);
+  return 0;
+}
+
+extern "C" int cortex_score_batch(void *state, const int *tokens, int batch, int n_tok, const int *slots,
+                                  const int *targets, double temperature, int top_k, float *logprob, float *entropy,
+                                  int *top_ids, float *top_logprob, int flags) {
+  clear_error();
+  if (!state) {
+    set_error("cortex_score_batch: state is NULL");
+    return -1;
+  }
+  Engine &e = *static_cast<Engine *>(state);
+  if (batch < 0 || n_tok < 0) {
+    set_error("negative batch or token count");
+    return -2;
+  }
+  if ((targets == nullptr) != (logprob == nullptr)) {
+    set_error("cortex_score_batch: targets and logprob go together");
+    return -2;
+  }
+  ScoreLaunch s;
+  s.rows = 0;  // checked before any token is fed
+  s.V = e.d.V;
+  s.ld = e.d.V;
+  s.n_tok = targets ? 1 : 0;
+  s.temperature = temperature;
+  s.top_k = top_k;
+  s.entropy = entropy;
+  int rc = check_score("cortex_score_batch", s);
+  if (rc) return rc;
+  if (top_k > 0 && (!top_ids || !top_logprob)) {
+    set_error("cortex_score_batch: NULL top_ids or top_logprob");
+    return -2;
+  }
+  if (batch == 0 || n_tok == 0) return 0;
+  if (!tokens) {
+    set_error("tokens is NULL");
+    return -2;
+  }
+  if (!slots_ok(e, slots, batch)) return -2;
+  const bool dev = flags & SNAI_DEVICE_PTRS;
+  DeviceGuard g(e.device);
+  rc = score_buffers(e);
+  if (rc) return rc;
+  const int R = score_rows_max(e);
+  std::vector<RowDesc> rows;
+  std::vector<size_t> at;  // the outputs' index of each row
+  rows.reserve((size_t)batch * n_tok);
+  at.reserve((size_t)batch * n_tok);
+  std::vector<int> done(batch, 0);
+  for (int b = 0; b < batch; ++b) {
+    const int sl = slots ? slots[b] : b;
+    for (int i = 0; i < n_tok && e.pos[sl] + i < e.d.ctx; ++i) {  // core/cortex.nim:495
+      const size_t idx = (size_t)b * n_tok + i;
+      rows.push_back(RowDesc{sl, e.pos[sl] + i, dev ? (int)idx : tokens[idx], (int)(rows.size() % R)});
+      at.push_back(idx);
+      done[b]++;
+    }
+  }
+  const cudaMemcpyKind out_kind = cudaMemcpyDeviceToHost;
+  for (size_t r0 = 0; r0 < rows.size(); r0 += R) {
+    const int n = (int)std::min<size_t>(R, rows.size() - r0);
+    float *slot_logits = e.logits;
+    e.logits = e.score_logits;  // the pass writes every row's logits there
+    rc = run_rows(e, rows.data() + r0, n, dev ? tokens : nullptr);
+    e.logits = slot_logits;
+    if (rc) return rc;
+    // runs of rows whose outputs are adjacent (one, unless a slot met ctx)
+    for (int i = 0; i < n;) {
+      int m = 1;
+      while (i + m < n && at[r0 + i + m] == at[r0 + i] + m) ++m;
+      const size_t o = at[r0 + i];
+      s.rows = m;
+      s.logits = e.score_logits + (size_t)i * e.d.V;
+      s.tokens = !targets ? nullptr : dev ? targets + o : e.score_tok;
+      s.logprob = !targets ? nullptr : dev ? logprob + o : e.score_lp;
+      s.entropy = !entropy ? nullptr : dev ? entropy + o : e.score_ent;
+      s.top_ids = !top_k ? nullptr : dev ? top_ids + o * top_k : e.score_ids;
+      s.top_logprob = !top_k ? nullptr : dev ? top_logprob + o * top_k : e.score_top;
+      if (targets && !dev &&
+          cudaMemcpyAsync(e.score_tok, targets + o, sizeof(int) * m, cudaMemcpyHostToDevice, e.stream) != cudaSuccess) {
+        set_error("target upload failed: %s", cudaGetErrorString(cudaGetLastError()));
+        return -4;
+      }
+      const int ptok = prof_begin(e);
+      rc = launch_score("cortex_score_batch", s, e.stream);
+      if (rc) return rc;
+      e.launches++;
+      prof_end(e, ptok, kProfScore, 4.0 * m * e.d.V + m * (8.0 * s.n_tok + 4.0 + 8.0 * top_k), 0.0);
+      if (!dev) {
+        bool ok = true;
+        auto back = [&](void *dst, const void *src, size_t bytes) {
+          ok = ok && cudaMemcpyAsync(dst, src, bytes, out_kind, e.stream) == cudaSuccess;
+        };
+        if (targets) back(logprob + o, e.score_lp, sizeof(float) * m);
+        if (entropy) back(entropy + o, e.score_ent, sizeof(float) * m);
+        if (top_k) back(top_ids + o * top_k, e.score_ids, sizeof(int) * (size_t)m * top_k);
+        if (top_k) back(top_logprob + o * top_k, e.score_top, sizeof(float) * (size_t)m * top_k);
+        if (!ok) {
+          set_error("score copy failed: %s", cudaGetErrorString(cudaGetLastError()));
+          return -4;
+        }
+      }
+      i += m;
+    }
+    // the last token's logits stay in the slot
+    for (int i = 0; i < n; ++i)
+      if (at[r0 + i] % n_tok == (size_t)n_tok - 1 &&
+          cudaMemcpyAsync(e.logits + (size_t)rows[r0 + i].slot * e.d.V, e.score_logits + (size_t)i * e.d.V,
+                          sizeof(float) * e.d.V, cudaMemcpyDeviceToDevice, e.stream) != cudaSuccess) {
+        set_error("logits copy failed");
+        return -4;
+      }
+  }
+  for (int b = 0; b < batch; ++b) {
+    const int sl = slots ? slots[b] : b;
+    e.pos[sl] += done[b];
+    if (done[b] == n_tok) e.logits_valid[sl] = 1;
+  }
+  return finish(e, !dev);
 }
 
 extern "C" int cortex_decode_batch(void *state, const int *slots, int batch, const float *uniforms,

@@ -39,6 +39,18 @@ class DeviceOnce {
   std::set<int> done_;
 };
 
+// Makes a device current for a scope.
+struct DeviceGuard {
+  int prev = -1, want;
+  explicit DeviceGuard(int d) : want(d) {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    if (prev != d) cudaSetDevice(d);
+  }
+  ~DeviceGuard() {
+    if (prev >= 0 && prev != want) cudaSetDevice(prev);
+  }
+};
+
 // Multiprocessor count of a device (queried once per device, thread-safe).
 int device_sm_count(int dev);
 
@@ -177,6 +189,11 @@ struct Engine {
   // host mirrors
   std::vector<int> pos;            // per slot
   std::vector<char> logits_valid;  // per slot
+  // scored positions (cortex_score_batch, made on first use): their logits,
+  // targets, log probabilities, entropies and alternatives
+  void *score_buf = nullptr;
+  float *score_logits = nullptr, *score_lp = nullptr, *score_ent = nullptr, *score_top = nullptr;
+  int *score_tok = nullptr, *score_ids = nullptr;
   TrainState *train = nullptr;     // gradients, Adam moments, training activations (made on first use)
   long long launches = 0;
 
@@ -196,7 +213,7 @@ struct Engine {
 // Kernel classes of the profiler (cortex_profile_read `kind`).
 enum ProfKind : int {
   kProfEmbed = 0, kProfNorm = 1, kProfQKV = 2, kProfAttention = 3, kProfWo = 4, kProfUp = 5, kProfDown = 6,
-  kProfLogits = 7, kProfSampler = 8, kProfPass = 9, kProfKinds = 10
+  kProfLogits = 7, kProfSampler = 8, kProfPass = 9, kProfScore = 10, kProfKinds = 11
 };
 // Brackets one launch: returns a token for prof_end (or -1 when off).
 int prof_begin(Engine &e);
@@ -258,6 +275,45 @@ int check_sample_args(const SampleLaunch &a);
 int decode_step_device(Engine &e, int batch, const SampleLaunch &sampler);
 int launch_sampler(const SampleLaunch &a, cudaStream_t stream);
 
+// ---- operators over rows of logits (score.cu) ----
+constexpr int kScoreMaxK = 512;  // ids in a row's lists: tokens, alternatives, teacher entries
+struct ScoreLaunch {
+  const void *logits = nullptr;
+  int dtype = 0;  // SNAI_DTYPE_*
+  int rows = 0, V = 0;
+  long long ld = 0;
+  const int *tokens = nullptr;
+  int n_tok = 0;
+  double temperature = 1.0;
+  int top_k = 0;
+  float *logprob = nullptr, *entropy = nullptr;
+  int *top_ids = nullptr;
+  float *top_logprob = nullptr;
+};
+struct DistillLaunch {
+  const void *logits = nullptr;
+  int dtype = 0;
+  int rows = 0, V = 0;
+  long long ld = 0;
+  const int *teacher_ids = nullptr;
+  const float *teacher_logits = nullptr;
+  int top_k = 0;
+  const int *labels = nullptr;
+  const float *row_grad = nullptr;
+  double temperature = 1.0, label_weight = 0.0;
+  int rest = 0;
+  float *loss = nullptr;
+  void *grad = nullptr;
+  long long grad_ld = 0;
+};
+// Check the arguments (`who` names the entry point in errors; pointers only
+// when there are rows); launch on `stream` of the device that holds the
+// arrays.  Return 0 or a negative error.
+int check_score(const char *who, const ScoreLaunch &s);
+int launch_score(const char *who, const ScoreLaunch &s, cudaStream_t stream);
+int check_distill(const char *who, const DistillLaunch &s);
+int launch_distill(const char *who, const DistillLaunch &s, cudaStream_t stream);
+
 // ---- merging and Net2Net (net2net.cu) ----
 constexpr int kMergeMaxSources = 64;
 struct MergeSources {
@@ -281,8 +337,11 @@ int train_moments(Engine &e);
 float *train_tensor(Engine &e, int which, const float *w);
 // Forward, loss and backward of core/cortex.nim:565-818 for act >= 1 tokens
 // (host arrays); gradients left in the gradient block, the mean loss in
-// *loss_out (synchronises).  Returns 0 or a negative error.
-int train_grads(Engine &e, const int *tin, const int *ttg, int act, float *loss_out);
+// *loss_out (synchronises).  With `distill` its loss takes the place of the
+// cross-entropy (its lists, constants and top_k are read; ttg are the labels
+// and may be NULL when they carry no weight).  Returns 0 or a negative error.
+int train_grads(Engine &e, const int *tin, const int *ttg, int act, float *loss_out,
+                const DistillLaunch *distill = nullptr);
 // Global-norm clip (1.0) and one Adam step with gradient divisor `scale`,
 // queued on e.stream.  Returns 0 or a negative error.
 int train_apply(Engine &e, float lr, float scale);

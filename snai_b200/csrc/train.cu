@@ -46,6 +46,7 @@
 #include <cstdio>
 #include <vector>
 
+#include "../../include/cortex.h"
 #include "common.cuh"
 #include "engine.h"
 #include "epilogue.cuh"
@@ -743,6 +744,8 @@ struct TrainState {
   float *dh = nullptr, *dn = nullptr, *dffn = nullptr, *datt = nullptr, *dqkv = nullptr, *gprod = nullptr;
   float *loss_rows = nullptr, *loss = nullptr, *clip = nullptr, *colpart = nullptr;
   int *prev = nullptr, *last = nullptr;
+  void *teach = nullptr;  // teacher lists of a distillation step: ids, then values ([rows][top_k] each)
+  size_t teach_cap = 0;   // entries of each
   double *clip_part = nullptr;
   // tensor-core engines (TF32 / BF16): transposed operands of the NN and TN
   // products -- a weight W^T, dY^T and X^T with the positions padded to Mp
@@ -935,6 +938,7 @@ void train_free(Engine &e) {
   cudaFree(e.train->mom);
   cudaFree(e.train->grad);
   cudaFree(e.train->act);
+  cudaFree(e.train->teach);
   delete e.train;
   e.train = nullptr;
 }
@@ -952,7 +956,7 @@ int train_adam_steps(const Engine &e) { return e.train ? e.train->adam_t : 0; }
 
 // Forward, loss and backward of one sequence (act >= 1 tokens, host arrays);
 // gradients are left in the gradient block; the mean loss goes to *loss_out.
-int train_grads(Engine &e, const int *tin, const int *ttg, int act, float *loss_out) {
+int train_grads(Engine &e, const int *tin, const int *ttg, int act, float *loss_out, const DistillLaunch *distill) {
   if (train_alloc(e)) return -1;
   TrainState &t = *e.train;
   const Dims &d = e.d;
@@ -961,7 +965,41 @@ int train_grads(Engine &e, const int *tin, const int *ttg, int act, float *loss_
   cudaStream_t st = e.stream;
   int rc = 0;
   rc |= cudaMemcpyAsync(t.tin, tin, sizeof(int) * act, cudaMemcpyHostToDevice, st) != cudaSuccess;
-  rc |= cudaMemcpyAsync(t.ttg, ttg, sizeof(int) * act, cudaMemcpyHostToDevice, st) != cudaSuccess;
+  if (ttg) rc |= cudaMemcpyAsync(t.ttg, ttg, sizeof(int) * act, cudaMemcpyHostToDevice, st) != cudaSuccess;
+  DistillLaunch ds;
+  if (distill) {
+    ds = *distill;
+    const size_t n = (size_t)act * ds.top_k;
+    if (n > t.teach_cap) {
+      if (cudaStreamSynchronize(st) != cudaSuccess) rc = 1;  // an earlier step may still read the old lists
+      cudaFree(t.teach);
+      t.teach = nullptr;
+      t.teach_cap = 0;
+      if (cudaMalloc(&t.teach, n * 8) != cudaSuccess) {
+        cudaGetLastError();
+        t.teach = nullptr;
+        set_error("device allocation of the teacher lists failed (%zu B)", n * 8);
+        return -1;
+      }
+      t.teach_cap = n;
+    }
+    int *ids = static_cast<int *>(t.teach);
+    float *vals = reinterpret_cast<float *>(ids + t.teach_cap);
+    rc |= cudaMemcpyAsync(ids, ds.teacher_ids, sizeof(int) * n, cudaMemcpyHostToDevice, st) != cudaSuccess;
+    rc |= cudaMemcpyAsync(vals, ds.teacher_logits, sizeof(float) * n, cudaMemcpyHostToDevice, st) != cudaSuccess;
+    ds.dtype = SNAI_DTYPE_FP32;
+    ds.rows = act;
+    ds.V = V;
+    ds.logits = t.probs;
+    ds.ld = t.Vp;
+    ds.teacher_ids = ids;
+    ds.teacher_logits = vals;
+    ds.labels = t.ttg;
+    ds.row_grad = nullptr;
+    ds.loss = t.loss_rows;
+    ds.grad = t.probs;  // in place, as the cross-entropy
+    ds.grad_ld = t.Vp;
+  }
   // the embedding gradient is accumulated; every other gradient is stored
   rc |= cudaMemsetAsync(mirror(e, t.grad, e.emb), 0, sizeof(float) * (size_t)V * D, st) != cudaSuccess;
   if (rc) {
@@ -1036,7 +1074,10 @@ int train_grads(Engine &e, const int *tin, const int *ttg, int act, float *loss_
   snai_train_rmsnorm<<<M, kRowThreads, 0, st>>>(t.hid[L], e.rms_final, t.nfinal, D);
   e.launches++;
   rc |= nt(V, D, t.nfinal, e.w_out, ET{ET::kStore, t.probs, nullptr, nullptr, t.Vp}, SimtStore{t.probs, t.Vp, 0});
-  snai_train_xent<<<M, kRowThreads, 0, st>>>(t.probs, V, t.Vp, t.ttg, t.loss_rows);
+  if (!distill)
+    snai_train_xent<<<M, kRowThreads, 0, st>>>(t.probs, V, t.Vp, t.ttg, t.loss_rows);
+  else if (launch_distill("cortex_distill_grads", ds, st))  // the rows' padding columns stay zero
+    return -1;
   snai_train_loss_sum<<<1, 32, 0, st>>>(t.loss_rows, M, t.loss);
   e.launches += 2;
   // the reference's training forward leaves its K/V rows in the cache

@@ -7,11 +7,12 @@ src/snai_inference.php:113-215.  Everything numeric happens in the library;
 this module only moves arguments across the C ABI.
 """
 import ctypes
+from typing import Any, NamedTuple
 
 import numpy as np
 
 from . import _lib
-from ._lib import CortexError, SampleParams, check, load
+from ._lib import CortexError, DistillParams, SampleParams, check, load
 from .modelgen import read_header
 
 VARIANT_A = 0  # src/snai_inference.php sampler
@@ -23,6 +24,20 @@ def sample_params(variant, temperature, rep_penalty, top_k=40, top_p=0.9, nan_gu
         nan_guard = 1 if variant == VARIANT_A else 0
     return SampleParams(int(variant), float(temperature), float(rep_penalty), int(top_k), float(top_p),
                         int(nan_guard))
+
+
+def distill_params(temperature=1.0, label_weight=0.0, rest=False):
+    return DistillParams(float(temperature), float(label_weight), 1 if rest else 0)
+
+
+class Score(NamedTuple):
+    """What a model says about given tokens: their log probabilities, the
+    rows' entropies (nats), the alternatives and their log probabilities."""
+
+    logprob: Any = None
+    entropy: Any = None
+    top_ids: Any = None
+    top_logprob: Any = None
 
 
 def _ptr(a):
@@ -120,6 +135,29 @@ class Cortex:
                                            ctypes.c_void_p(ids_dev.data_ptr()), _lib.DEVICE_PTRS),
               "cortex_decode_steps")
 
+    def score(self, tokens, targets=None, temperature=1.0, top_k=0, slots=None):
+        """Feeds tokens [B, n] as `forward` does and scores every position:
+        after token i, the log probability of targets[b, i], the entropy and
+        the top_k alternatives.  Returns a Score of [B, n] arrays (alternatives
+        [B, n, top_k]; positions past ctx keep zeros, their ids -1)."""
+        t = np.ascontiguousarray(np.atleast_2d(tokens), dtype=np.int32)
+        B, n = t.shape
+        tg = None if targets is None else np.ascontiguousarray(np.atleast_2d(targets), dtype=np.int32)
+        if tg is not None and tg.shape != t.shape:
+            raise CortexError(f"targets {tg.shape} do not match the tokens {t.shape}")
+        sl = None if slots is None else np.ascontiguousarray(slots, dtype=np.int32)
+        if sl is not None and len(sl) != B:
+            raise CortexError(f"{len(sl)} slots for {B} rows of tokens")
+        k = int(top_k)
+        lp = None if tg is None else np.zeros((B, n), dtype=np.float32)
+        ent = np.zeros((B, n), dtype=np.float32)
+        ids = np.full((B, n, k), -1, dtype=np.int32) if k > 0 else None
+        top = np.zeros((B, n, k), dtype=np.float32) if k > 0 else None
+        opt = lambda a: None if a is None else _ptr(a)  # noqa: E731
+        check(self.lib.cortex_score_batch(self.h, _ptr(t), B, n, opt(sl), opt(tg), float(temperature), k, opt(lp),
+                                          _ptr(ent), opt(ids), opt(top), _lib.HOST_PTRS), "cortex_score_batch")
+        return Score(lp, ent, ids, top)
+
     def logits(self, slots):
         s = np.ascontiguousarray(slots, dtype=np.int32)
         out = np.zeros((len(s), self.vocab), dtype=np.float32)
@@ -155,7 +193,8 @@ class Cortex:
         n = self.slots if s is None else len(s)
         check(self.lib.cortex_seq_rewind(self.h, None if s is None else _ptr(s), n, int(pos)), "cortex_seq_rewind")
 
-    PROFILE_KINDS = ("embed", "rmsnorm", "qkv", "attention", "wo", "up", "down", "logits", "sampler", "pass")
+    PROFILE_KINDS = ("embed", "rmsnorm", "qkv", "attention", "wo", "up", "down", "logits", "sampler", "pass",
+                     "score")
 
     def profile(self, on=True):
         check(self.lib.cortex_profile_enable(self.h, 1 if on else 0), "cortex_profile_enable")
@@ -191,6 +230,33 @@ class Cortex:
         loss = ctypes.c_float(0.0)
         check(self.lib.cortex_train_grads(self.h, _ptr(a), _ptr(b), len(a), ctypes.byref(loss)), "cortex_train_grads")
         return float(loss.value)
+
+    def distill_grads(self, inputs, teacher_ids, teacher_logits, labels=None, temperature=1.0, label_weight=0.0,
+                      rest=False):
+        """cortex_distill_grads: forward + backward against a teacher's top
+        logits [n, k] (ids of -1 pad a list); the mean loss.  Gradients stay on
+        the device for train_apply."""
+        a = np.ascontiguousarray(inputs, dtype=np.int32)
+        ids = np.ascontiguousarray(teacher_ids, dtype=np.int32)
+        vals = np.ascontiguousarray(teacher_logits, dtype=np.float32)
+        y = None if labels is None else np.ascontiguousarray(labels, dtype=np.int32)
+        if ids.ndim != 2 or ids.shape != vals.shape or len(ids) != len(a) or (y is not None and len(y) != len(a)):
+            raise CortexError(f"inputs {a.shape}, teacher lists {ids.shape} / {vals.shape} and labels do not match")
+        prm = distill_params(temperature, label_weight, rest)
+        loss = ctypes.c_float(0.0)
+        check(self.lib.cortex_distill_grads(self.h, _ptr(a), _ptr(ids), _ptr(vals), ids.shape[1],
+                                            None if y is None else _ptr(y), len(a), ctypes.byref(prm),
+                                            ctypes.byref(loss)), "cortex_distill_grads")
+        return float(loss.value)
+
+    def distill_step(self, inputs, teacher_ids, teacher_logits, lr, labels=None, temperature=1.0, label_weight=0.0,
+                     rest=False):
+        """distill_grads, then the clip and Adam step of `train_step`; the mean loss."""
+        loss = self.distill_grads(inputs, teacher_ids, teacher_logits, labels, temperature, label_weight, rest)
+        act = min(len(inputs), self.ctx)
+        if act > 0:
+            self.train_apply(lr, act)
+        return loss
 
     def train_apply(self, lr, scale):
         check(self.lib.cortex_train_apply(self.h, float(lr), float(scale)), "cortex_train_apply")
@@ -293,6 +359,136 @@ def sample_device(logits_dev, uniforms_dev, params, hist_dev=None, hist_len_dev=
                             ctypes.c_void_p(uniforms_dev.data_ptr()), ctypes.byref(params),
                             ctypes.c_void_p(out_dev.data_ptr()), ctypes.c_void_p(stream)), "cortex_sample")
     return out_dev
+
+
+def _dev_rows(logits):
+    """(dtype code, rows, vocab, row stride) of device logits [rows, vocab]."""
+    if logits.dim() != 2 or not logits.is_cuda:
+        raise CortexError("logits must be a 2-d CUDA tensor")
+    code = _DTYPES.get(str(logits.dtype))
+    if code is None:
+        raise CortexError(f"logits of type {logits.dtype}: float32, bfloat16 or float16 are taken")
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise CortexError("the elements of a row of logits must be adjacent")
+    return code, rows, vocab, logits.stride(0) if rows > 1 else max(vocab, logits.stride(0))
+
+
+_DTYPES = {"torch.float32": _lib.DTYPE_FP32, "torch.bfloat16": _lib.DTYPE_BF16, "torch.float16": _lib.DTYPE_FP16}
+
+
+def _dev_arg(name, t, logits, shape, dtype):
+    """The address of a dense device argument, None when absent."""
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape) or str(t.dtype) != dtype or t.device != logits.device or not t.is_contiguous():
+        raise CortexError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {logits.device} is needed, "
+                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _dev_tokens(tokens, logits, rows):
+    """(address, tokens a row) of tokens [rows] or [rows, n]."""
+    if tokens is None:
+        return None, 0
+    if tokens.dim() not in (1, 2):
+        raise CortexError("tokens must be [rows] or [rows, n]")
+    n = 1 if tokens.dim() == 1 else tokens.shape[1]
+    return _dev_arg("tokens", tokens, logits, (rows,) if tokens.dim() == 1 else (rows, n), "torch.int32"), n
+
+
+def _stream_of(stream, device):
+    """The stream's handle, and the context that new tensors are made in."""
+    import contextlib
+
+    import torch
+
+    if stream is None:
+        return torch.cuda.current_stream(device).cuda_stream, contextlib.nullcontext()
+    return stream, torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
+
+
+def _dev_grad(logits, grad, rows, vocab):
+    import torch
+
+    if grad is None:
+        grad = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+    elif grad.shape != logits.shape or grad.dtype != logits.dtype or grad.device != logits.device or (
+            vocab > 1 and grad.stride(1) != 1):
+        raise CortexError("the gradient must have the logits' shape, type and device, its rows' elements adjacent")
+    return grad, grad.stride(0) if rows > 1 else max(vocab, grad.stride(0))
+
+
+def score_device(logits_dev, tokens_dev=None, temperature=1.0, top_k=0, want_entropy=True, stream=None):
+    """Log probabilities of tokens [rows] or [rows, n], entropies and the top_k
+    alternatives of device logits [rows, vocab] (cortex_score), as a Score of
+    device tensors.  Runs on `stream` (a handle), by default torch's current
+    stream of the logits' device."""
+    import torch
+
+    code, rows, vocab, ld = _dev_rows(logits_dev)
+    tok, n = _dev_tokens(tokens_dev, logits_dev, rows)
+    k = int(top_k)
+    handle, made_in = _stream_of(stream, logits_dev.device)
+    dev = logits_dev.device
+    with made_in:
+        lp = None if tok is None else torch.empty(tokens_dev.shape, dtype=torch.float32, device=dev)
+        ent = torch.empty(rows, dtype=torch.float32, device=dev) if want_entropy else None
+        ids = torch.empty((rows, k), dtype=torch.int32, device=dev) if k > 0 else None
+        top = torch.empty((rows, k), dtype=torch.float32, device=dev) if k > 0 else None
+    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    check(load().cortex_score(logits_dev.data_ptr(), code, rows, vocab, ld, tok, n, float(temperature), k, at(lp),
+                              at(ent), at(ids), at(top), handle), "cortex_score")
+    return Score(lp, ent, ids, top)
+
+
+def score_grad_device(logits_dev, tokens_dev=None, g_logprob_dev=None, g_entropy_dev=None, temperature=1.0,
+                      grad_dev=None, stream=None):
+    """The gradient of sum(g_logprob * logprob) + sum(g_entropy * entropy) of
+    score_device with respect to the logits (cortex_score_grad); grad_dev may
+    be the logits themselves."""
+    code, rows, vocab, ld = _dev_rows(logits_dev)
+    tok, n = _dev_tokens(tokens_dev, logits_dev, rows)
+    if (tokens_dev is None) != (g_logprob_dev is None):
+        raise CortexError("tokens and g_logprob go together")
+    gl = _dev_arg("g_logprob", g_logprob_dev, logits_dev, tokens_dev.shape if tokens_dev is not None else (),
+                  "torch.float32")
+    ge = _dev_arg("g_entropy", g_entropy_dev, logits_dev, (rows,), "torch.float32")
+    handle, made_in = _stream_of(stream, logits_dev.device)
+    with made_in:
+        grad, gld = _dev_grad(logits_dev, grad_dev, rows, vocab)
+    check(load().cortex_score_grad(logits_dev.data_ptr(), code, rows, vocab, ld, tok, n, float(temperature), gl, ge,
+                                   grad.data_ptr(), gld, handle), "cortex_score_grad")
+    return grad
+
+
+def distill_device(logits_dev, teacher_ids_dev, teacher_logits_dev, labels=None, temperature=1.0, label_weight=0.0,
+                   rest=False, row_grad=None, want_grad=True, grad_dev=None, stream=None):
+    """The distillation loss of device logits [rows, vocab] against a teacher's
+    top logits [rows, k] (cortex_distill), and the gradient of
+    sum(row_grad * loss), which may take the logits' place (grad_dev).
+    Returns (loss [rows], gradient or None)."""
+    import torch
+
+    code, rows, vocab, ld = _dev_rows(logits_dev)
+    if teacher_ids_dev.dim() != 2:
+        raise CortexError("teacher_ids must be [rows, k]")
+    k = teacher_ids_dev.shape[1]
+    ids = _dev_arg("teacher_ids", teacher_ids_dev, logits_dev, (rows, k), "torch.int32")
+    vals = _dev_arg("teacher_logits", teacher_logits_dev, logits_dev, (rows, k), "torch.float32")
+    y = _dev_arg("labels", labels, logits_dev, (rows,), "torch.int32")
+    rg = _dev_arg("row_grad", row_grad, logits_dev, (rows,), "torch.float32")
+    prm = distill_params(temperature, label_weight, rest)
+    handle, made_in = _stream_of(stream, logits_dev.device)
+    grad, gld = None, 0
+    with made_in:
+        loss = torch.empty(rows, dtype=torch.float32, device=logits_dev.device)
+        if want_grad:
+            grad, gld = _dev_grad(logits_dev, grad_dev, rows, vocab)
+    check(load().cortex_distill(logits_dev.data_ptr(), code, rows, vocab, ld, ids, vals, k, y, rg, ctypes.byref(prm),
+                                loss.data_ptr(), None if grad is None else grad.data_ptr(), gld, handle),
+          "cortex_distill")
+    return loss, grad
 
 
 class SnaiCortexBridge:
