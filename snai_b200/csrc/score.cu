@@ -7,13 +7,27 @@
 // e_i = exp(d_i) and S = sum e_i:
 //   log p_i = d_i - log S,  entropy H = log S - sum(e_i d_i) / S.
 // A masked logit (-inf) has e_i = 0 and takes no gradient; a row holding a
-// NaN or +inf has no distribution and yields NaN (its alternatives' ids -1).
+// NaN or +inf has no distribution: its S is NaN and so is all that follows
+// (its alternatives' ids -1).
+//
+// All three read a row once from memory and are bound by that (and by the
+// gradient's one write).  A row lives in shared memory, cut into slices over
+// a cluster of CTAs when it is long: 16-byte words copied asynchronously,
+// each by the thread that will read it, so no barrier stands between a copy
+// and its use, and the next row's copies go out as soon as a thread is done
+// with its words.  Pass A gathers m, S and sum(e d) together (a running
+// maximum per thread, checked once per chunk of four words); what comes
+// after it - alternatives, gradient - reads shared memory only.
 #include <cuda_fp16.h>
 
 #include <algorithm>
 #include <cfloat>
+#include <climits>
 #include <cmath>
 #include <initializer_list>
+#include <map>
+#include <mutex>
+#include <tuple>
 #include <utility>
 
 #include "../../include/cortex.h"
@@ -23,24 +37,160 @@
 namespace snai {
 namespace {
 
-constexpr int kThreads = 512;
 constexpr int kMaxList = kScoreMaxK;
-constexpr int kMaxVocab = 1 << 19; // as cortex_sample
+constexpr int kMaxVocab = 1 << 19;  // as cortex_sample
+constexpr int kStages = 4;          // copy groups a row's words are committed in
+constexpr int kChunk = 4;           // words a thread takes at a time
+constexpr float kLowest = -200.f;   // exponents (base 2) are cut here: 2^-200 is 0 in fp32, and 0 * d stays 0
+constexpr float kLn2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+// ---- small device pieces ----
 
-// maximum that keeps a NaN
+// maxima that keep a NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// two floats in a register pair
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f2 v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float sum2(f2 v) {
+  float a, b;
+  unpack2(v, a, b);
+  return a + b;
+}
+
+// A 16-byte word of logits: kN elements; kMasked is -inf in each of its 32-bit parts.
+template <typename E> struct Word;
+template <> struct Word<float> {
+  static constexpr int kN = 4;
+  static constexpr unsigned kMasked = 0xff800000u;
+  __device__ static __forceinline__ void unpack(const uint4 &w, f2 *v) {
+    v[0] = pack2(__uint_as_float(w.x), __uint_as_float(w.y));
+    v[1] = pack2(__uint_as_float(w.z), __uint_as_float(w.w));
+  }
+  __device__ static __forceinline__ uint4 pack(const f2 *v) {
+    float a, b, c, d;
+    unpack2(v[0], a, b);
+    unpack2(v[1], c, d);
+    return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
+  }
+  // maximum over kChunk words
+  __device__ static __forceinline__ float max(const uint4 *q) {
+    float m = __uint_as_float(q[0].x);
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      m = max_nan(m, max_nan(__uint_as_float(q[j].x), __uint_as_float(q[j].y)));
+      m = max_nan(m, max_nan(__uint_as_float(q[j].z), __uint_as_float(q[j].w)));
+    }
+    return m;
+  }
+  __device__ static __forceinline__ float one(const float *p) { return *p; }
+  __device__ static __forceinline__ void put(float *p, float v) { *p = v; }
+};
+template <> struct Word<__nv_bfloat16> {
+  static constexpr int kN = 8;
+  static constexpr unsigned kMasked = 0xff80ff80u;
+  __device__ static __forceinline__ f2 two(unsigned x) {
+    return pack2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  }
+  __device__ static __forceinline__ unsigned two(f2 v) {
+    float a, b;
+    unpack2(v, a, b);
+    unsigned r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+  }
+  __device__ static __forceinline__ void unpack(const uint4 &w, f2 *v) {
+    v[0] = two(w.x), v[1] = two(w.y), v[2] = two(w.z), v[3] = two(w.w);
+  }
+  __device__ static __forceinline__ uint4 pack(const f2 *v) {
+    return make_uint4(two(v[0]), two(v[1]), two(v[2]), two(v[3]));
+  }
+  __device__ static __forceinline__ unsigned max2(unsigned a, unsigned b) {
+    unsigned r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ static __forceinline__ float max(const uint4 *q) {
+    unsigned m = q[0].x;
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) m = max2(m, max2(max2(q[j].x, q[j].y), max2(q[j].z, q[j].w)));
+    return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  }
+  __device__ static __forceinline__ float one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+  __device__ static __forceinline__ void put(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+};
+template <> struct Word<__half> {
+  static constexpr int kN = 8;
+  static constexpr unsigned kMasked = 0xfc00fc00u;
+  __device__ static __forceinline__ f2 two(unsigned x) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x));
+    return pack2(f.x, f.y);
+  }
+  __device__ static __forceinline__ unsigned two(f2 v) {
+    float a, b;
+    unpack2(v, a, b);
+    unsigned r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+  }
+  __device__ static __forceinline__ void unpack(const uint4 &w, f2 *v) {
+    v[0] = two(w.x), v[1] = two(w.y), v[2] = two(w.z), v[3] = two(w.w);
+  }
+  __device__ static __forceinline__ uint4 pack(const f2 *v) {
+    return make_uint4(two(v[0]), two(v[1]), two(v[2]), two(v[3]));
+  }
+  __device__ static __forceinline__ unsigned max2(unsigned a, unsigned b) {
+    unsigned r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ static __forceinline__ float max(const uint4 *q) {
+    unsigned m = q[0].x;
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) m = max2(m, max2(max2(q[j].x, q[j].y), max2(q[j].z, q[j].w)));
+    float a, b;
+    unpack2(two(m), a, b);
+    return max_nan(a, b);
+  }
+  __device__ static __forceinline__ float one(const __half *p) { return __half2float(*p); }
+  __device__ static __forceinline__ void put(__half *p, float v) { *p = __float2half_rn(v); }
+};
 
 // Sort key of a logit and its id: descending value, then ascending id.
 __device__ __forceinline__ unsigned long long sort_key(float z, int id) {
@@ -48,246 +198,828 @@ __device__ __forceinline__ unsigned long long sort_key(float z, int id) {
   const unsigned k = (unsigned)b ^ (b < 0 ? 0xffffffffu : 0x80000000u);
   return ((unsigned long long)k << 32) | (unsigned)~id;
 }
-
-template <typename F>
-__device__ __forceinline__ auto block_reduce(decltype(F::id()) v, decltype(F::id()) *red) {
-  for (int o = 16; o > 0; o >>= 1) v = F::op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < (int)(blockDim.x >> 5); ++w) v = F::op(v, red[w]);
-  return v;
+__device__ __forceinline__ float key_logit(unsigned long long key) {
+  const unsigned k = (unsigned)(key >> 32);
+  return __uint_as_float(k ^ (k & 0x80000000u ? 0x80000000u : 0xffffffffu));
 }
-struct MaxOp {
-  __device__ static float id() { return -FLT_MAX; }
-  __device__ static float op(float a, float b) { return max_nan(a, b); }
-};
-struct SumOp {
-  __device__ static float id() { return 0.f; }
-  __device__ static float op(float a, float b) { return a + b; }
-};
-struct SumD {
-  __device__ static double id() { return 0.0; }
-  __device__ static double op(double a, double b) { return a + b; }
-};
-struct SumI {
-  __device__ static int id() { return 0; }
-  __device__ static int op(int a, int b) { return a + b; }
-};
+__device__ __forceinline__ int key_id(unsigned long long key) { return (int)~(unsigned)key; }
 
-struct ScoreArgs {
+// ---- rows in shared memory ----
+
+struct Rows {
   const void *logits;
   long long ld;
   int rows, V;
+  int wps;  // words of a slice
+  int C;    // CTAs of a cluster, one slice each
+};
+
+// One CTA's slice of one row: words [first, first + n) of the row's 16-byte
+// grid, which starts `pad` elements before the row when the row does not
+// start on a word.  Thread t owns words t, t + NT, ... of the slice.
+template <typename E, int NT>
+struct Slice {
+  static constexpr int kN = Word<E>::kN;
+  const E *row;  // the row's element 0
+  int pad, first, n, V;
+
+  __device__ __forceinline__ void set(const Rows &a, int r, unsigned rank) {
+    row = static_cast<const E *>(a.logits) + (long long)r * a.ld;
+    pad = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(E));
+    V = a.V;
+    first = (int)rank * a.wps;
+    n = min(a.wps, (pad + V + kN - 1) / kN - first);
+  }
+  // id of element 0 of local word w (negative in the leading pad)
+  __device__ __forceinline__ int id0(int w) const { return (first + w) * kN - pad; }
+  __device__ __forceinline__ bool whole(int w) const {
+    const int i = id0(w);
+    return i >= 0 && i + kN <= V;
+  }
+  // local element index of an id, or -1 when another slice holds it
+  __device__ __forceinline__ int local(int id) const {
+    const int e = id + pad - first * kN;
+    return e >= 0 && e < n * kN ? e : -1;
+  }
+  // Copies this thread's words of stage st (cps chunks) into buf and commits
+  // them.  The row's ragged ends are filled up with -inf.
+  __device__ __forceinline__ void load(int st, int cps, uint4 *buf) const {
+    for (int c = st * cps; c < (st + 1) * cps; ++c)
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        const int w = (c * kChunk + j) * NT + (int)threadIdx.x;
+        if (w >= n) break;
+        if (whole(w))
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(buf + w)), "l"(row + id0(w))
+                       : "memory");
+        else
+          ragged(w, buf);
+      }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __noinline__ void ragged(int w, uint4 *buf) const {
+    E *p = reinterpret_cast<E *>(buf + w);
+    const int i0 = id0(w);
+    for (int k = 0; k < kN; ++k) Word<E>::put(p + k, i0 + k >= 0 && i0 + k < V ? Word<E>::one(row + i0 + k) : -INFINITY);
+  }
+  __device__ __noinline__ void store_ragged(int w, uint4 q, E *out) const {
+    const E *p = reinterpret_cast<const E *>(&q);
+    const int i0 = id0(w);
+    for (int k = 0; k < kN; ++k)
+      if (i0 + k >= 0 && i0 + k < V) out[i0 + k] = p[k];
+  }
+  // this thread's four words of chunk c (all masked past the slice's end)
+  __device__ __forceinline__ void chunk(int c, const uint4 *buf, uint4 *q) const {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      const int w = (c * kChunk + j) * NT + (int)threadIdx.x;
+      const unsigned k = Word<E>::kMasked;
+      q[j] = w < n ? buf[w] : make_uint4(k, k, k, k);
+    }
+  }
+};
+
+template <int N> __device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// ---- softmax statistics ----
+
+// m, S = sum 2^((z - m) c) and, when asked, W = sum 2^x x (x = (z - m) c) and
+// S1 = sum 2^((z - m) log2 e), the sum at temperature 1.  All masked: m is
+// the lowest float and S 0.  A NaN or +inf makes S NaN.
+struct Stat {
+  float m, s, w, s1;
+};
+__device__ __forceinline__ float cut(float x) { return max_nan(x, kLowest); }
+
+// a's sums relative to the maximum m >= a.m
+template <bool W, bool S1>
+__device__ __forceinline__ void rebase(Stat &a, float m, float c) {
+  const float x = cut((a.m - m) * c), f = ex2(x);
+  if (W) a.w = f * fmaf(a.s, x, a.w);
+  a.s *= f;
+  if (S1) a.s1 *= ex2(cut((a.m - m) * kLog2E));
+  a.m = m;
+}
+
+template <typename E, bool W, bool S1>
+struct Running {
+  float m = -FLT_MAX;
+  f2 s = 0, w = 0, s1 = 0;
+
+  __device__ __forceinline__ void add(const uint4 *q, float cm, float c) {
+    if (!(cm <= m)) {  // a new maximum, or a NaN
+      const float nm = max_nan(m, cm), x = cut((m - nm) * c), f = ex2(x);
+      const f2 ff = pack2(f, f);
+      if (W) w = mul2(ff, fma2(s, pack2(x, x), w));
+      s = mul2(ff, s);
+      if (S1) {
+        const float f1 = ex2(cut((m - nm) * kLog2E));
+        s1 = mul2(pack2(f1, f1), s1);
+      }
+      m = nm;
+    }
+    const f2 nm2 = pack2(-m, -m), c2 = pack2(c, c), l2 = pack2(kLog2E, kLog2E);
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      f2 v[Word<E>::kN / 2];
+      Word<E>::unpack(q[j], v);
+#pragma unroll
+      for (int k = 0; k < Word<E>::kN / 2; ++k) {
+        const f2 d = add2(v[k], nm2);
+        f2 x = mul2(d, c2);
+        float a, b;
+        unpack2(x, a, b);
+        if (W) {
+          a = cut(a), b = cut(b);
+          x = pack2(a, b);
+        }
+        const f2 e = pack2(ex2(a), ex2(b));
+        s = add2(s, e);
+        if (W) w = fma2(e, x, w);
+        if (S1) {
+          unpack2(mul2(d, l2), a, b);
+          s1 = add2(s1, pack2(ex2(a), ex2(b)));
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ Stat get() const { return {m, sum2(s), W ? sum2(w) : 0.f, S1 ? sum2(s1) : 0.f}; }
+};
+
+// Combines the statistics of n lanes (a power of two; lanes of equal number
+// modulo n hold the same ones); every lane gets the result.
+template <bool W, bool S1>
+__device__ __forceinline__ Stat combine_lanes(Stat a, int n, float c) {
+  rebase<W, S1>(a, warp_max_nan(a.m), c);
+  for (int o = n / 2; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    if (W) a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
+    if (S1) a.s1 += __shfl_xor_sync(0xffffffffu, a.s1, o);
+  }
+  return a;
+}
+__device__ __forceinline__ Stat no_stat() { return {-FLT_MAX, 0.f, 0.f, 0.f}; }
+
+// What a CTA tells the others of its cluster about its slice.
+struct __align__(16) Slip {
+  Stat st;
+  double v[6];  // sums over the entries of a list (row gradients)
+  int count;    // alternatives in its list (scores)
+};
+
+__device__ __forceinline__ Stat peer_stat(const Slip *mine, unsigned rank) {
+  const uint32_t p = mapa_shared(smem_u32(mine), rank);
+  return {__uint_as_float(ld_cluster_u32(p)), __uint_as_float(ld_cluster_u32(p + 4)),
+          __uint_as_float(ld_cluster_u32(p + 8)), __uint_as_float(ld_cluster_u32(p + 12))};
+}
+
+// ---- scores ----
+
+struct ScoreArgs {
+  Rows in;
   const int *tokens;
   int n_tok;
-  float inv_t;
-  int top_k;
+  float c, inv_t;  // log2(e) / T, 1 / T
+  int top_k, cap;  // cap: candidates the buffer holds (a power of two)
   float *logprob, *entropy;
   int *top_ids;
   float *top_logprob;
 };
 
-template <typename E>
-__global__ void __launch_bounds__(kThreads) snai_score(const ScoreArgs a) {
-  __shared__ float redf[32];
-  __shared__ int redi[32];
-  __shared__ unsigned long long cand[kMaxList];
-  __shared__ int n_cand;
-  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const E *z = static_cast<const E *>(a.logits) + (long long)r * a.ld;
-    float m = -FLT_MAX;
-    for (int i = threadIdx.x; i < a.V; i += kThreads) m = max_nan(m, to_f(z[i]));
-    m = block_reduce<MaxOp>(m, redf);
-    float s = 0.f, w = 0.f;
-    for (int i = threadIdx.x; i < a.V; i += kThreads) {
-      const float d = max_nan((to_f(z[i]) - m) * a.inv_t, -150.f), e = __expf(d);
-      s += e;
-      w += e * d;
-    }
-    s = block_reduce<SumOp>(s, redf);
-    w = block_reduce<SumOp>(w, redf);
-    const bool bad = !(s < INFINITY);
-    const float ls = logf(s);
-    for (int j = threadIdx.x; j < a.n_tok; j += kThreads) {
-      const int t = a.tokens[(long long)r * a.n_tok + j];
-      a.logprob[(long long)r * a.n_tok + j] =
-          t < 0 || t >= a.V ? 0.f : bad ? NAN : s == 0.f ? -INFINITY : (to_f(z[t]) - m) * a.inv_t - ls;
-    }
-    if (threadIdx.x == 0 && a.entropy) a.entropy[r] = bad ? NAN : s == 0.f ? 0.f : ls - w / s;
-    if (!a.top_k) continue;
-    int *ids = a.top_ids + (long long)r * a.top_k;
-    float *lps = a.top_logprob + (long long)r * a.top_k;
-    if (bad) {
-      for (int j = threadIdx.x; j < a.top_k; j += kThreads) ids[j] = -1, lps[j] = NAN;
-      continue;
-    }
-    // the k-th largest key by bisection over the 64-bit keys
-    unsigned long long lo = 0, hi = ~0ull;  // count(>= lo) >= k
-    while (lo < hi) {
-      const unsigned long long mid = lo + (hi - lo) / 2 + 1;
-      int c = 0;
-      for (int i = threadIdx.x; i < a.V; i += kThreads) c += sort_key(to_f(z[i]), i) >= mid;
-      if (block_reduce<SumI>(c, redi) >= a.top_k)
-        lo = mid;
-      else
-        hi = mid - 1;
-    }
-    if (threadIdx.x == 0) n_cand = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.V; i += kThreads) {
-      const unsigned long long k = sort_key(to_f(z[i]), i);
-      if (k >= lo) cand[atomicAdd(&n_cand, 1)] = k;
-    }
-    __syncthreads();
-    for (int j = threadIdx.x; j < a.top_k; j += kThreads) {
-      int rank = 0;
-      for (int l = 0; l < a.top_k; ++l) rank += cand[l] > cand[j];
-      const int id = (int)~(unsigned)cand[j];
-      ids[rank] = id;
-      lps[rank] = s == 0.f ? -INFINITY : (to_f(z[id]) - m) * a.inv_t - ls;
-    }
-    __syncthreads();
-  }
+__device__ __forceinline__ float log_p(float z, float m, float inv_t, float s, float ls) {
+  return s == 0.f || z == -INFINITY ? -INFINITY + (s - s) : (z - m) * inv_t - ls;
 }
 
+// The k-th largest of the groups' maxima (n values in shared memory), or a
+// little less, by one warp: at least k of the groups reach it, so at least k
+// elements do.  -inf when there are fewer groups than k.
+__device__ __forceinline__ float kth_of_maxima(const float *g, int n, int k) {
+  if (n < k) return -INFINITY;
+  const int lane = threadIdx.x & 31;
+  auto ordered = [](float v) {
+    const int b = __float_as_int(v);
+    return b ^ ((b >> 31) & 0x7fffffff);
+  };
+  int lo = 0x7fffffff, hi = (int)0x80000000;
+  for (int i = lane; i < n; i += 32) {
+    const int v = ordered(g[i]);
+    lo = min(lo, v), hi = max(hi, v);
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  // at least k groups reach lo
+  const int slack = k + (k >> 2) + 2;
+  while (lo < hi) {
+    const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) >> 1);
+    int c = 0;
+    for (int i = lane; i < n; i += 32) c += ordered(g[i]) >= mid;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= k) {
+      lo = mid;
+      if (c <= slack) break;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  return __int_as_float(lo ^ ((lo >> 31) & 0x7fffffff));
+}
+
+template <typename E, int NT, bool TOPK, bool ENT>
+__global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreArgs a) {
+  constexpr int NW = NT / 32;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ Stat part[2][NW];
+  __shared__ Slip slip[2];
+  __shared__ float tau;
+  __shared__ int n_cand, n_ge;
+  uint4 *buf = reinterpret_cast<uint4 *>(smem);
+  // alternatives: candidates, then (clusters) the slice's sorted list, the maxima of the chunks and of the threads
+  unsigned long long *cand = reinterpret_cast<unsigned long long *>(smem + (size_t)a.in.wps * 16);
+  unsigned long long *list = cand + a.cap;
+  float *cmax = reinterpret_cast<float *>(list + (a.in.C > 1 ? a.top_k : 0));
+  const int t = threadIdx.x, lane = t & 31, wid = t >> 5;
+  const int C = a.in.C;
+  const unsigned rank = C > 1 ? cluster_ctarank() : 0;
+  const int step = gridDim.x / C;
+  const int chunks = (a.in.wps + kChunk * NT - 1) / (kChunk * NT), cps = (chunks + kStages - 1) / kStages;
+  float *tmax = cmax + chunks * NT;
+
+  Slice<E, NT> cur, nxt;
+  int r = blockIdx.x / C;
+  cur.set(a.in, r, rank);
+  for (int s = 0; s < kStages; ++s) cur.load(s, cps, buf);
+  int par = 0;
+  for (; r < a.in.rows; r += step, par ^= 1) {
+    const bool more = r + step < a.in.rows;
+    if (more) nxt.set(a.in, r + step, rank);
+    // the tokens' logits, read beside the row's copies
+    float zt[kMaxList / NT];
+    bool in[kMaxList / NT];
+    if (rank == 0)
+#pragma unroll
+      for (int i = 0; i < kMaxList / NT; ++i) {
+        const int j = i * NT + t;
+        zt[i] = 0.f, in[i] = false;
+        if (j < a.n_tok) {
+          const int id = a.tokens[(long long)r * a.n_tok + j];
+          in[i] = id >= 0 && id < a.in.V;
+          if (in[i]) zt[i] = Word<E>::one(cur.row + id);
+        }
+      }
+    // pass A
+    Running<E, ENT, false> run;
+    float tm = -INFINITY;
+    auto stage = [&](int s) {
+      for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
+        uint4 q[kChunk];
+        cur.chunk(c, buf, q);
+        const float cm = Word<E>::max(q);
+        run.add(q, cm, a.c);
+        if (TOPK) {
+          cmax[c * NT + t] = cm;
+          tm = max_nan(tm, cm);
+        }
+      }
+      if (!TOPK && more) nxt.load(s, cps, buf);
+    };
+    if (!TOPK && more) {  // one group of the next row follows each stage
+      copies_wait<kStages - 1>(), stage(0);
+      copies_wait<kStages - 1>(), stage(1);
+      copies_wait<kStages - 1>(), stage(2);
+      copies_wait<kStages - 1>(), stage(3);
+    } else {
+      copies_wait<3>(), stage(0);
+      copies_wait<2>(), stage(1);
+      copies_wait<1>(), stage(2);
+      copies_wait<0>(), stage(3);
+    }
+    if (TOPK) tmax[t] = tm;
+    Stat st = combine_lanes<ENT, false>(run.get(), 32, a.c);
+    if (lane == 0) part[par][wid] = st;
+    __syncthreads();
+    st = combine_lanes<ENT, false>(part[par][lane % NW], NW, a.c);
+    const bool bad_slice = st.s != st.s;
+    const int kl = TOPK ? max(0, min(a.top_k, min(cur.V, cur.id0(cur.n)) - max(0, cur.id0(0)))) : 0;
+    if (TOPK) {
+      // a lower bound of the slice's kl-th largest logit: from the threads'
+      // maxima when those are many more than kl, else from the chunks'
+      if (wid == 0) {
+        const bool few = 4 * kl <= NT;
+        const float b = bad_slice || kl == 0 ? INFINITY : kth_of_maxima(few ? tmax : cmax, few ? NT : chunks * NT, kl);
+        if (lane == 0) tau = b, n_cand = 0;
+      }
+      __syncthreads();
+    }
+    if (C > 1) {
+      if (t == 0) slip[par].st = st, slip[par].count = bad_slice ? 0 : kl;
+      cluster_sync_all();
+      st = combine_lanes<ENT, false>(lane % 16 < C ? peer_stat(&slip[par], lane % 16) : no_stat(), 16, a.c);
+    }
+    const float ls = logf(st.s);
+    const bool bad = st.s != st.s;
+    if (rank == 0) {
+#pragma unroll
+      for (int i = 0; i < kMaxList / NT; ++i) {
+        const int j = i * NT + t;
+        if (j < a.n_tok)
+          a.logprob[(long long)r * a.n_tok + j] = in[i] ? log_p(zt[i], st.m, a.inv_t, st.s, ls) : 0.f;
+      }
+      if (ENT && t == 0 && a.entropy) a.entropy[r] = st.s == 0.f ? 0.f : ls - kLn2 * st.w / st.s;
+    }
+    if (TOPK) {
+      // candidates: this thread's elements that reach tau
+      const float b = tau;
+      auto each = [&](float least, auto f) {  // f(z, id) for own elements of chunks whose maximum reaches `least`
+        for (int c = 0; c < chunks; ++c) {
+          if (!(cmax[c * NT + t] >= least)) continue;
+          for (int j = 0; j < kChunk; ++j) {
+            const int w = (c * kChunk + j) * NT + t;
+            if (w >= cur.n) break;
+            const E *p = reinterpret_cast<const E *>(buf + w);
+            const int i0 = cur.id0(w);
+            for (int k = 0; k < Word<E>::kN; ++k) {
+              const float z = Word<E>::one(p + k);
+              if (z >= least && i0 + k >= 0 && i0 + k < cur.V) f(z, i0 + k);
+            }
+          }
+        }
+      };
+      if (tm >= b)
+        each(b, [&](float z, int id) {
+          const int i = atomicAdd(&n_cand, 1);
+          if (i < a.cap) cand[i] = sort_key(z, id);
+        });
+      __syncthreads();
+      int n = n_cand;
+      if (n > a.cap) {
+        // too many (ties, few groups): bisect over whole keys to between kl and cap of them
+        unsigned long long lo = sort_key(b, INT_MAX), hi = ~0ull;
+        for (;;) {
+          const unsigned long long mid = lo + ((hi - lo) >> 1) + 1;
+          __syncthreads();
+          if (t == 0) n_ge = 0, n_cand = 0;
+          __syncthreads();
+          int cnt = 0;
+          each(key_logit(mid), [&](float z, int id) { cnt += sort_key(z, id) >= mid; });
+          cnt = __reduce_add_sync(0xffffffffu, cnt);
+          if (lane == 0) atomicAdd(&n_ge, cnt);
+          __syncthreads();
+          n = n_ge;
+          if (n < kl) {
+            hi = mid - 1;
+          } else {
+            lo = mid;
+            if (n <= a.cap) break;
+          }
+        }
+        each(key_logit(lo), [&](float z, int id) {
+          const unsigned long long k = sort_key(z, id);
+          if (k >= lo) cand[atomicAdd(&n_cand, 1)] = k;
+        });
+        __syncthreads();
+      }
+      if (more)
+        for (int s = 0; s < kStages; ++s) nxt.load(s, cps, buf);
+      // order them: by counting when they are few, else a bitonic sort
+      auto place = [&](int at, unsigned long long key) {
+        if (C > 1) {
+          list[at] = key;
+        } else {
+          a.top_ids[(long long)r * a.top_k + at] = key_id(key);
+          a.top_logprob[(long long)r * a.top_k + at] = log_p(key_logit(key), st.m, a.inv_t, st.s, ls);
+        }
+      };
+      if (n <= 192) {
+        for (int i = t; i < n; i += NT) {
+          const unsigned long long key = cand[i];
+          int above = 0;
+          for (int j = 0; j < n; ++j) above += cand[j] > key;
+          if (above < kl) place(above, key);
+        }
+      } else {
+        int len = 256;
+        while (len < n) len *= 2;
+        for (int i = n + t; i < len; i += NT) cand[i] = 0;
+        for (int size = 2; size <= len; size *= 2)
+          for (int stride = size / 2; stride > 0; stride /= 2) {
+            __syncthreads();
+            for (int i = t; i < len / 2; i += NT) {
+              const int x = 2 * i - (i & (stride - 1)), y = x + stride;
+              const unsigned long long u = cand[x], v = cand[y];
+              if ((u < v) == ((x & size) == 0)) cand[x] = v, cand[y] = u;
+            }
+          }
+        __syncthreads();
+        for (int i = t; i < kl; i += NT) place(i, cand[i]);
+      }
+      if (C > 1) {
+        // an entry's place among all slices: its own plus the greater ones of every other list
+        cluster_sync_all();
+        for (int i = t; i < (bad ? 0 : kl); i += NT) {
+          const unsigned long long key = list[i];
+          int at = i;
+          for (int o = 1; o < C; ++o) {
+            const unsigned peer = (rank + o) % C;
+            const uint32_t pl = mapa_shared(smem_u32(list), peer);
+            int x = 0, y = (int)ld_cluster_u32(mapa_shared(smem_u32(&slip[par].count), peer));
+            while (x < y) {
+              const int h = (x + y) / 2;
+              if (ld_cluster_u64(pl + 8 * h) > key)
+                x = h + 1;
+              else
+                y = h;
+            }
+            at += x;
+          }
+          if (at < a.top_k) {
+            a.top_ids[(long long)r * a.top_k + at] = key_id(key);
+            a.top_logprob[(long long)r * a.top_k + at] = log_p(key_logit(key), st.m, a.inv_t, st.s, ls);
+          }
+        }
+      }
+      if (bad && rank == 0)
+        for (int i = t; i < a.top_k; i += NT)
+          a.top_ids[(long long)r * a.top_k + i] = -1, a.top_logprob[(long long)r * a.top_k + i] = NAN;
+    }
+    cur = nxt;
+  }
+  if (C > 1) cluster_sync_all();  // others may still read this CTA's slip and list
+}
+
+// ---- row gradients ----
+
 struct RowGradArgs {
-  const void *logits;
-  long long ld;
-  int rows, V;
-  const int *ids;  // [rows][n] tokens or teacher ids
+  Rows in;
+  const int *ids;     // [rows][n] tokens, or teacher ids
+  const float *vals;  // [rows][n] their gradients, or teacher values
   int n;
-  const float *vals;  // [rows][n] g_logprob or teacher logits
-  float inv_t;
-  double inv_td;
+  float c;           // log2(e) / T
+  float inv_t_f;
+  double inv_t;      // 1 / T
   const float *g_entropy;
   const int *labels;
   const float *row_grad;
-  float t, t2, a;  // temperature, temperature^2, label weight
+  double t, a;  // temperature, label weight
   int rest;
   float *loss;
   void *grad;
   long long grad_ld;
 };
 
-// MODE 0: the gradient of scores; MODE 1: distillation.
-template <typename E, int MODE>
-__global__ void __launch_bounds__(kThreads) snai_row_grad(const RowGradArgs a) {
-  __shared__ float redf[32];
-  __shared__ double redd[32];
-  __shared__ int redi[32];
-  __shared__ int ids[kMaxList];
-  __shared__ double q[kMaxList];   // weights (MODE 0: g)
-  __shared__ double lq[kMaxList];
-  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const E *z = static_cast<const E *>(a.logits) + (long long)r * a.ld;
-    E *gr = a.grad ? static_cast<E *>(a.grad) + (long long)r * a.grad_ld : nullptr;
-    int valid = 0;
-    __syncthreads();
-    for (int j = threadIdx.x; j < a.n; j += kThreads) {
-      const int id = a.ids[(long long)r * a.n + j];
-      const bool in = id >= 0 && id < a.V;
-      ids[j] = in ? id : -1;
-      valid += in;
-      q[j] = in ? (double)a.vals[(long long)r * a.n + j] : 0.0;
+__device__ __forceinline__ double warp_sum_d(double v) {
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Sums over the entries of a row's list (see snai_row_grad).
+constexpr int kSums = 6;
+struct Entries {
+  double kl, qs;   // sum of q (log q - d), and of q, over the entries in the slice
+  double q;        // sum of q (MODE 0: of the token gradients) over the list
+  double se, se1;  // exponentials of the listed logits, at T and at temperature 1
+  double zy;       // the label's logit
+  __device__ __forceinline__ void add(const double *v) {
+    kl += v[0], qs += v[1], q += v[2], se += v[3], se1 += v[4], zy += v[5];
+  }
+  __device__ __forceinline__ void put(double *v) const {
+    v[0] = kl, v[1] = qs, v[2] = q, v[3] = se, v[4] = se1, v[5] = zy;
+  }
+  // over the warp
+  __device__ __forceinline__ void sum(bool rest, bool label1) {
+    kl = warp_sum_d(kl), qs = warp_sum_d(qs), q = warp_sum_d(q), zy = warp_sum_d(zy);
+    if (rest) se = warp_sum_d(se);
+    if (rest && label1) se1 = warp_sum_d(se1);
+  }
+};
+
+__device__ __forceinline__ void copy4(void *dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+// first(j): no earlier entry of the list names the same id.
+__device__ __forceinline__ bool is_first(const int *ids, int j) {
+  const int id = ids[j];
+  const int4 *v = reinterpret_cast<const int4 *>(ids);
+  bool seen = false;
+  int l = 0;
+  for (; l + 4 <= j; l += 4) {
+    const int4 x = v[l >> 2];
+    seen |= x.x == id || x.y == id || x.z == id || x.w == id;
+  }
+  for (; l < j; ++l) seen |= ids[l] == id;
+  return !seen;
+}
+
+// MODE 0: the gradient of scores.  With x_i = d_i / ln 2, G the sum of the
+// row's token gradients and g_H the entropy's (EXTRA: when there is one):
+//   grad_i = e_i (alpha + beta x_i) + (sum of g_j of the tokens equal to i) / T,
+//   alpha = (g_H ln2 W / S - G) / (S T),  beta = -g_H ln2 / (S T).
+// MODE 1: distillation, q_j the teacher's weights:
+//   grad_i = e_i alpha + gamma softmax(z)_i - what the list and the label take.
+// EXTRA: labels at T != 1, whose softmax needs exponentials of its own.  With
+// `rest` the listed logits are taken out of the staged row, so that the
+// unlisted mass is a sum of its own (1 - the listed would lose a confident
+// student's); the list's part is summed separately.
+// Pass B writes the terms every element has; after a barrier the threads that
+// hold the entries write their ids' gradients.  An id listed more than once
+// is handled by its first entry, in the order of the list: no atomics.
+// The entries' weights and the loss are held in 64 bits: a handful of values
+// a row, and a loss that is a small difference of large terms.
+template <typename E, int NT, int MODE, bool EXTRA>
+__global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_row_grad(const RowGradArgs a) {
+  constexpr int NW = NT / 32, kN = Word<E>::kN;
+  constexpr bool ENT = MODE == 0 && EXTRA, LABEL1 = MODE == 1 && EXTRA;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ Stat part[2][NW];
+  __shared__ float tch_m[NW], tch_s[NW];  // the teacher's list, by warp: maximum, sum of exponentials
+  __shared__ double sums[NW][kSums];
+  __shared__ Slip slip[2];
+  __shared__ float scal[2];  // g_entropy or row_grad of the row
+  uint4 *buf = reinterpret_cast<uint4 *>(smem);
+  const bool rest = MODE == 1 && a.rest, soft = MODE == 1 && !a.rest;
+  const int n = a.n, ne = n + (MODE == 1 && a.labels ? 1 : 0), cap = (ne + 3) & ~3;
+  // lists: ids and values of two rows, then weights and logits of this one
+  int *ids2 = reinterpret_cast<int *>(smem + (size_t)a.in.wps * 16);
+  float *vals2 = reinterpret_cast<float *>(ids2 + 2 * cap);
+  float *wt = vals2 + 2 * cap, *zl = wt + cap;
+  const int t = threadIdx.x, lane = t & 31, wid = t >> 5;
+  const int C = a.in.C;
+  const unsigned rank = C > 1 ? cluster_ctarank() : 0;
+  const int step = gridDim.x / C;
+  const int chunks = (a.in.wps + kChunk * NT - 1) / (kChunk * NT), cps = (chunks + kStages - 1) / kStages;
+  const int nwl = min((ne + 31) / 32, NW);  // warps that hold entries
+
+  Slice<E, NT> cur, nxt;
+  int r = blockIdx.x / C, par = 0;
+  // a row's lists are committed with its first stage
+  auto load = [&](const Slice<E, NT> &s, int row, int p, int st) {
+    if (st == 0) {
+      for (int j = t; j < n; j += NT) {
+        copy4(ids2 + p * cap + j, a.ids + (long long)row * n + j);
+        copy4(vals2 + p * cap + j, a.vals + (long long)row * n + j);
+      }
+      if (ne > n && t == n % NT) copy4(ids2 + p * cap + n, a.labels + row);
+      if (t == 0) {
+        if (ENT) copy4(&scal[p], a.g_entropy + row);
+        if (MODE == 1 && a.row_grad) copy4(&scal[p], a.row_grad + row);
+      }
     }
-    valid = block_reduce<SumI>(valid, redi);
-    const int y = MODE == 1 && a.labels && a.labels[r] >= 0 && a.labels[r] < a.V ? a.labels[r] : -1;
-    const float gh = MODE == 0 && a.g_entropy ? a.g_entropy[r] : 0.f;
-    if (!valid && y < 0 && gh == 0.f) {  // a row of padding
-      if (MODE == 1 && threadIdx.x == 0) a.loss[r] = 0.f;
-      if (gr)
-        for (int i = threadIdx.x; i < a.V; i += kThreads) gr[i] = from_f<E>(0.f);
+    s.load(st, cps, buf);
+  };
+  cur.set(a.in, r, rank);
+  for (int s = 0; s < kStages; ++s) load(cur, r, 0, s);
+  for (; r < a.in.rows; r += step, par ^= 1) {
+    const bool more = r + step < a.in.rows;
+    if (more) nxt.set(a.in, r + step, rank);
+    const int *ids = ids2 + par * cap;
+    const float *vals = vals2 + par * cap;
+    const int V = a.in.V;
+    auto valid = [&](int id) { return id >= 0 && id < V; };
+    auto here = [&](int id) { return valid(id) && cur.local(id) >= 0; };  // in this slice
+    auto staged = [&](int id) { return reinterpret_cast<E *>(buf) + cur.local(id); };
+    bool any = false;  // anything but padding in the row?  (own entries, once they have landed)
+    auto look = [&] {
+      for (int j = t; j < ne; j += NT) any |= valid(ids[j]);
+      if (ENT && t == 0) any |= scal[par] != 0.f;
+    };
+    if (rest) {
+      copies_wait<0>();
+      look();
+      any = __syncthreads_or(any);
+      for (int j = t; j < ne; j += NT)
+        if (here(ids[j])) zl[j] = Word<E>::one(staged(ids[j]));
+      __syncthreads();
+      for (int j = t; j < n; j += NT)
+        if (here(ids[j])) Word<E>::put(staged(ids[j]), -INFINITY);
+      __syncthreads();
+    }
+    // pass A
+    Running<E, ENT, LABEL1> run;
+    auto stage = [&](int s) {
+      for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
+        uint4 q[kChunk];
+        cur.chunk(c, buf, q);
+        run.add(q, Word<E>::max(q), a.c);
+      }
+    };
+    copies_wait<3>(), stage(0);
+    copies_wait<2>(), stage(1);
+    copies_wait<1>(), stage(2);
+    copies_wait<0>(), stage(3);
+    Stat st = combine_lanes<ENT, LABEL1>(run.get(), 32, a.c);
+    if (lane == 0) part[par][wid] = st;
+    if (soft && wid < nwl) {
+      float m = -INFINITY, s = 0.f;
+      for (int j = t; j < n; j += NT)
+        if (valid(ids[j])) m = max_nan(m, vals[j]);
+      m = warp_max_nan(m);
+      for (int j = t; j < n; j += NT)
+        if (valid(ids[j]) && vals[j] != -INFINITY) s += expf((vals[j] - m) * a.inv_t_f);
+      s = warp_sum(s);
+      if (lane == 0) tch_m[wid] = m, tch_s[wid] = s;
+    }
+    if (rest) {
+      __syncthreads();
+    } else {
+      look();
+      any = __syncthreads_or(any);
+    }
+    st = combine_lanes<ENT, LABEL1>(part[par][lane % NW], NW, a.c);
+    if (rest) {  // the listed logits may hold the slice's maximum
+      float m = -INFINITY;
+      for (int j = lane; j < n; j += 32)
+        if (here(ids[j])) m = max_nan(m, zl[j]);
+      rebase<ENT, LABEL1>(st, max_nan(st.m, warp_max_nan(m)), a.c);
+    }
+    // the entries' weights, and the sums over them
+    Entries own = {};
+    unsigned firsts = 0;
+    bool twice = false;
+    if (wid < nwl) {
+      double lse = 0;
+      if (soft) {
+        float m = -INFINITY, s = 0.f;
+        for (int w = 0; w < nwl; ++w) m = max_nan(m, tch_m[w]);
+        for (int w = 0; w < nwl; ++w)
+          if (tch_m[w] != -INFINITY) s += tch_s[w] * expf((tch_m[w] - m) * a.inv_t_f);
+        lse = m == -INFINITY ? 0.0 : m * a.inv_t + (double)logf(s);
+      }
+      for (int j = t, i = 0; j < ne; j += NT, ++i) {
+        const int id = ids[j];
+        const bool in = here(id);
+        if (in && !rest) zl[j] = Word<E>::one(staged(id));
+        if (valid(id)) {
+          if (is_first(ids, j))
+            firsts |= 1u << i;
+          else
+            twice = true;
+        }
+        double q = 0;
+        if (MODE == 1 && j == n) {
+          if (in) own.zy = zl[j];
+        } else if (MODE == 0) {
+          if (valid(id)) q = vals[j];
+        } else if (valid(id) && vals[j] != -INFINITY) {
+          const double lq = rest ? (double)vals[j] : vals[j] * a.inv_t - lse;
+          q = rest ? exp(lq) : (double)expf((float)lq);
+          if (in && q != 0.0) {
+            own.kl += q * (lq - ((double)zl[j] - st.m) * a.inv_t);
+            own.qs += q;
+          }
+        }
+        own.q += q;
+        if (rest && in && j < n && (firsts >> i & 1)) {
+          own.se += ex2(cut((zl[j] - st.m) * a.c));
+          if (LABEL1) own.se1 += ex2(cut((zl[j] - st.m) * kLog2E));
+        }
+        wt[j] = (float)q;
+      }
+      own.sum(rest, LABEL1);
+      if (lane == 0) own.put(sums[wid]);
+    }
+    const bool dups = __syncthreads_or(twice);
+    Entries tot = {};
+    for (int w = 0; w < nwl; ++w) tot.add(sums[w]);
+    if (C > 1) {
+      if (t == 0) {
+        slip[par].st = st;
+        tot.put(slip[par].v);
+      }
+      cluster_sync_all();
+      const double q_all = tot.q;  // every slice has seen the whole list
+      const Stat mine = lane % 16 < C ? peer_stat(&slip[par], lane % 16) : no_stat();
+      st = combine_lanes<ENT, LABEL1>(mine, 16, a.c);
+      tot = {};
+      if (lane < C) {
+        double v[kSums];
+        const uint32_t p = mapa_shared(smem_u32(slip[par].v), lane);
+        for (int k = 0; k < kSums; ++k) v[k] = ld_cluster_f64(p + 8 * k);
+        tot.add(v);
+        // d of the listed, and their exponentials, relative to the row's maximum
+        if (tot.qs > 0) tot.kl += tot.qs * (((double)st.m - mine.m) * a.inv_t);
+        tot.se *= ex2(cut((mine.m - st.m) * a.c));
+        tot.se1 *= ex2(cut((mine.m - st.m) * kLog2E));
+      }
+      tot.sum(rest, LABEL1);
+      tot.q = q_all;
+    }
+    // the row's scalars
+    const float S = rest ? st.s + (float)tot.se : st.s;
+    const float S1 = LABEL1 ? (rest ? st.s1 + (float)tot.se1 : st.s1) : S;
+    const float inv_s = S == 0.f ? 0.f : 1.f / S;
+    const int y = ne > n && valid(ids[n]) ? ids[n] : -1;
+    float alpha, beta = 0.f, gamma = 0.f, kt = 0.f, mass = 0.f, ru = 0.f, ky = 0.f;
+    if (MODE == 0) {
+      const float gh = ENT ? scal[par] : 0.f, k = inv_s * a.inv_t_f;
+      alpha = -(float)tot.q * k;
+      if (ENT) alpha += gh * kLn2 * st.w * inv_s * k, beta = -gh * kLn2 * k;
+    } else {
+      const double rr = rest && st.s > 0.f ? fmax(0.0, 1.0 - tot.q) : 0.0;
+      const float rg = a.row_grad ? scal[par] : 1.f;
+      mass = (float)(tot.q + rr);
+      ru = rr > 0.0 ? (float)rr * (S / st.s) : 0.f;  // the teacher's rest over the student's
+      kt = rg * (float)((1.0 - a.a) * a.t);
+      ky = y >= 0 ? rg * (float)a.a : 0.f;
+      alpha = kt * (mass - ru) * inv_s;
+      if (LABEL1)
+        gamma = S1 == 0.f ? 0.f : ky / S1;
+      else
+        alpha += ky * inv_s;
+      if (t == 0 && rank == 0) {
+        double l = 0;
+        if (a.a < 1.0) {
+          l = S == 0.f ? (tot.q > 0 ? INFINITY : 0.0) : tot.kl + tot.q * log((double)S);
+          if (rr > 0.0) l += rr * (log(rr) + log1p(tot.se / st.s));
+          l *= (1.0 - a.a) * a.t * a.t;
+        }
+        if (y >= 0) l += a.a * (tot.zy == -INFINITY ? INFINITY : st.m - tot.zy + log((double)S1));
+        a.loss[r] = !any ? 0.f : S != S ? NAN : (float)l;
+      }
+    }
+    if (!a.grad) {
+      if (more)
+        for (int s = 0; s < kStages; ++s) load(nxt, r + step, par ^ 1, s);
+      cur = nxt;
       continue;
     }
-    float m = -FLT_MAX;
-    for (int i = threadIdx.x; i < a.V; i += kThreads) m = max_nan(m, to_f(z[i]));
-    m = block_reduce<MaxOp>(m, redf);
-    auto listed = [&](int i) {
-      for (int j = 0; j < a.n; ++j)
-        if (ids[j] == i) return true;
-      return false;
-    };
-    float s = 0.f, w = 0.f, s1 = 0.f, u = 0.f;
-    for (int i = threadIdx.x; i < a.V; i += kThreads) {
-      const float zi = to_f(z[i]), d = max_nan((zi - m) * a.inv_t, -150.f), e = __expf(d);
-      s += e;
-      w += e * d;
-      if (MODE == 1) s1 += __expf(max_nan(zi - m, -150.f));
-      if (MODE == 1 && a.rest && !listed(i)) u += e;
-    }
-    s = block_reduce<SumOp>(s, redf);
-    w = block_reduce<SumOp>(w, redf);
-    s1 = block_reduce<SumOp>(s1, redf);
-    u = block_reduce<SumOp>(u, redf);
-    const float ls = logf(s), inv_s = s > 0.f ? 1.f / s : s == 0.f ? 0.f : NAN;
-    float gsum = 0.f, cr = 0.f, mass = 0.f;
-    const float wy = y >= 0 ? a.a : 0.f;
-    if (MODE == 0) {
-      float g = 0.f;
-      for (int j = threadIdx.x; j < a.n; j += kThreads) g += (float)q[j];
-      gsum = block_reduce<SumOp>(g, redf);
-    } else {
-      double tm = -INFINITY;
-      for (int j = 0; j < a.n; ++j)
-        if (ids[j] >= 0) tm = fmax(tm, q[j]);
-      if (tm == -INFINITY) tm = 0;  // a list without mass
-      double ts = 0;
-      for (int j = threadIdx.x; j < a.n; j += kThreads)
-        if (ids[j] >= 0) ts += exp((q[j] - tm) * a.inv_td);
-      ts = block_reduce<SumD>(ts, redd);
-      double kl = 0, qs = 0;
-      for (int j = threadIdx.x; j < a.n; j += kThreads) {
-        lq[j] = a.rest ? q[j] : (q[j] - tm) * a.inv_td - log(ts);
-        const double qj = ids[j] >= 0 && q[j] != -INFINITY ? exp(lq[j]) : 0.0;
-        q[j] = qj;
-        if (qj > 0) {
-          const double zj = to_f(z[ids[j]]);
-          kl += qj * (lq[j] - (zj == -INFINITY ? zj : (zj - m) * a.inv_td - log((double)s)));
+    // pass B
+    E *out = static_cast<E *>(a.grad) + (long long)r * a.grad_ld;
+    const bool vec = ((reinterpret_cast<uintptr_t>(out) - cur.pad * sizeof(E)) & 15) == 0;
+    const f2 nm2 = pack2(-st.m, -st.m), c2 = pack2(a.c, a.c), l2 = pack2(kLog2E, kLog2E);
+    const f2 al2 = pack2(alpha, alpha), be2 = pack2(beta, beta), ga2 = pack2(gamma, gamma);
+#pragma unroll 1
+    for (int s = 0; s < kStages; ++s) {
+      for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
+        uint4 q[kChunk];
+        cur.chunk(c, buf, q);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          f2 v[kN / 2];
+          Word<E>::unpack(q[j], v);
+#pragma unroll
+          for (int k = 0; k < kN / 2; ++k) {
+            const f2 d = add2(v[k], nm2);
+            f2 x = mul2(d, c2);
+            float u, w;
+            unpack2(x, u, w);
+            if (ENT) {
+              u = cut(u), w = cut(w);
+              x = pack2(u, w);
+            }
+            const f2 e = pack2(ex2(u), ex2(w));
+            v[k] = mul2(e, ENT ? fma2(x, be2, al2) : al2);
+            if (LABEL1) {
+              unpack2(mul2(d, l2), u, w);
+              v[k] = fma2(pack2(ex2(u), ex2(w)), ga2, v[k]);
+            }
+          }
+          q[j] = any ? Word<E>::pack(v) : make_uint4(0u, 0u, 0u, 0u);
         }
-        qs += qj;
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          const int w = (c * kChunk + j) * NT + t;
+          if (w < cur.n) {
+            const int i0 = cur.id0(w);
+            if (vec && cur.whole(w))
+              *reinterpret_cast<uint4 *>(out + i0) = q[j];
+            else
+              cur.store_ragged(w, q[j], out);
+          }
+        }
       }
-      kl = block_reduce<SumD>(kl, redd);
-      qs = block_reduce<SumD>(qs, redd);
-      double rr = 0;
-      if (a.rest && valid && u > 0.f) {
-        rr = fmax(0.0, 1.0 - qs);
-        if (rr > 0) kl += rr * (log(rr) - log((double)u / s));
-        cr = (float)(rr / u);
-      }
-      mass = (float)(qs + rr);
-      if (threadIdx.x == 0) {
-        double l = a.a < 1.f ? (1.0 - a.a) * a.t2 * kl : 0.0;
-        const double zy = y >= 0 ? to_f(z[y]) : 0.f;
-        if (y >= 0) l -= a.a * (zy == -INFINITY ? zy : zy - m - log((double)s1));
-        a.loss[r] = inv_s != inv_s ? NAN : (float)l;
-      }
+      if (more) load(nxt, r + step, par ^ 1, s);
     }
-    if (!gr) continue;
-    const float rg = MODE == 1 && a.row_grad ? a.row_grad[r] : 1.f;
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.V; i += kThreads) {
-      const float zi = to_f(z[i]), d = max_nan((zi - m) * a.inv_t, -150.f), e = __expf(d);
-      float g = 0.f;
-      if (MODE == 0) {
-        float hot = 0.f;
-        for (int j = 0; j < a.n; ++j)
-          if (ids[j] == i) hot += (float)q[j];
-        const float p = e * inv_s;
-        g = (hot - p * gsum - gh * p * (d - w * inv_s)) * a.inv_t;
-      } else {
-        double hot = 0;
-        bool on = false;
-        for (int j = 0; j < a.n; ++j)
-          if (ids[j] == i) hot += q[j], on = true;
-        g = (1.f - a.a) * a.t * (e * mass * inv_s - (float)hot - (on ? 0.f : e * cr));
-        if (y >= 0) g += wy * (__expf(max_nan(zi - m, -150.f)) / s1 - (i == y ? 1.f : 0.f));
-        g *= rg;
-      }
-      gr[i] = from_f<E>(zi == -INFINITY ? (inv_s != inv_s ? NAN : 0.f) : inv_s != inv_s ? NAN : g);
+    if (ne > 0) {
+      __syncthreads();  // the listed ids' gradients, over the base written by their words' owners
+      if (any)
+        for (int j = t, i = 0; j < ne; j += NT, ++i) {
+          const int id = ids[j];
+          if (!(firsts >> i & 1) || cur.local(id) < 0) continue;
+          float q = wt[j];
+          if (dups)
+            for (int l = j + 1; l < n; ++l)
+              if (ids[l] == id) q += wt[l];
+          const float z = zl[j], d = z - st.m;
+          float g;
+          if (MODE == 0) {
+            const float x = cut(d * a.c);
+            g = ex2(x) * fmaf(x, beta, alpha) + q * a.inv_t_f;
+          } else {
+            const float p = ex2(cut(d * a.c)) * inv_s;
+            g = kt * (j < n ? mass * p - q : (mass - ru) * p);
+            if (y >= 0) {
+              const float p1 = LABEL1 ? ex2(cut(d * kLog2E)) / S1 : p;
+              g += ky * (id == y ? p1 - 1.f : p1);
+            }
+          }
+          Word<E>::put(out + id, S != S ? NAN : z == -INFINITY ? 0.f : g);
+        }
     }
+    cur = nxt;
   }
+  if (C > 1) cluster_sync_all();  // others may still read this CTA's slip
 }
 
 // ---------------------------------------------------------------------------
@@ -389,21 +1121,118 @@ int check_grad(const char *who, const void *logits, int dtype, int rows, int voc
   return -2;
 }
 
-int launched(const char *who) {
-  const cudaError_t e = cudaGetLastError();
+// How rows are cut and spread.
+struct Plan {
+  int wps, C, nt;
+};
+
+// A row's slices hold at most 66 KB: three CTAs of an SM then have a row
+// each in flight or in work.  Longer rows go over a cluster of up to 8 CTAs,
+// then (few can be that long) slices grow to what one CTA can hold, then the
+// cluster to 16.  With fewer rows than SMs a row is spread further, down to
+// slices of 8 KB.
+Plan plan_rows(const void *logits, int dtype, int rows, int vocab, long long ld, size_t extra, int sms) {
+  const int es = elem_size(dtype), kn = 16 / es;
+  const bool pitch = ld * es % 16 == 0;
+  const int pad = pitch ? (int)((reinterpret_cast<uintptr_t>(logits) & 15) / es) : kn - 1;
+  const int words = (pad + vocab + kn - 1) / kn;
+  const size_t bytes = (size_t)words * 16, best = 66 * 1024, most = 224 * 1024 - extra;
+  int C = (int)std::min<size_t>((bytes + best - 1) / best, 8);
+  if ((bytes + C - 1) / C > most) C = 16;
+  while (C <= 4 && rows * C * 2 <= sms && bytes / (2 * C) >= 8192) C *= 2;
+  Plan p;
+  p.C = C;
+  p.wps = (words + C - 1) / C;
+  p.nt = p.wps <= 1024 ? 128 : 256;
+  return p;
+}
+
+// Launches `kern` over the rows with as many clusters as fit the GPU at once
+// (asked once per kernel, device and shape), or as many as there are rows.
+template <class A>
+int launch_rows(const char *who, void (*kern)(A), const A &args, int nt, size_t smem, int dev, cudaStream_t stream) {
+  const void *fn = reinterpret_cast<const void *>(kern);
+  const int C = args.in.C;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)C;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(nt);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = C > 1 ? 1 : 0;
+  cfg.gridDim = dim3((unsigned)C);
+  static std::mutex mu;
+  static std::map<std::tuple<const void *, int, int, size_t>, int> fits;
+  int fit = 0;
+  {
+    std::lock_guard<std::mutex> g(mu);
+    int &f = fits[std::make_tuple(fn, dev, C, smem)];
+    if (f == 0) {
+      bool ok = set_dyn_smem(kern, 227 * 1024);
+      ok = ok && cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, 100) == cudaSuccess;
+      if (C > 8) ok = ok && cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+      if (C > 1) {
+        ok = ok && cudaOccupancyMaxActiveClusters(&f, fn, &cfg) == cudaSuccess;
+      } else {
+        ok = ok && cudaOccupancyMaxActiveBlocksPerMultiprocessor(&f, fn, nt, smem) == cudaSuccess;
+        f *= device_sm_count(dev);
+      }
+      if (!ok || f < 1) {
+        f = 0;
+        set_error("%s: rows of %d logits do not fit this GPU: %s", who, args.in.V, cudaGetErrorString(cudaGetLastError()));
+        return -4;
+      }
+    }
+    fit = f;
+  }
+  cfg.gridDim = dim3((unsigned)(std::min(args.in.rows, fit) * C));
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args);
   if (e == cudaSuccess) return 0;
+  cudaGetLastError();
   set_error("%s launch failed: %s", who, cudaGetErrorString(e));
   return -4;
 }
 
 template <class F>
-void by_dtype(int dtype, F &&f) {
-  if (dtype == SNAI_DTYPE_FP32)
-    f(float());
-  else if (dtype == SNAI_DTYPE_BF16)
-    f(__nv_bfloat16());
-  else
-    f(__half());
+int by_dtype(int dtype, F &&f) {
+  if (dtype == SNAI_DTYPE_FP32) return f(float());
+  if (dtype == SNAI_DTYPE_BF16) return f(__nv_bfloat16());
+  return f(__half());
+}
+
+template <typename E, int NT>
+int score_nt(const char *who, const ScoreArgs &a, size_t smem, int dev, cudaStream_t st) {
+  if (a.top_k) return launch_rows(who, snai_score<E, NT, true, true>, a, NT, smem, dev, st);
+  if (a.entropy) return launch_rows(who, snai_score<E, NT, false, true>, a, NT, smem, dev, st);
+  return launch_rows(who, snai_score<E, NT, false, false>, a, NT, smem, dev, st);
+}
+
+// mode 0: scores' gradient, 1: distillation; extra: as the kernel's EXTRA
+template <typename E, int NT>
+int grad_nt(const char *who, const RowGradArgs &a, int mode, bool extra, size_t smem, int dev, cudaStream_t st) {
+  if (mode == 0)
+    return extra ? launch_rows(who, snai_row_grad<E, NT, 0, true>, a, NT, smem, dev, st)
+                 : launch_rows(who, snai_row_grad<E, NT, 0, false>, a, NT, smem, dev, st);
+  return extra ? launch_rows(who, snai_row_grad<E, NT, 1, true>, a, NT, smem, dev, st)
+               : launch_rows(who, snai_row_grad<E, NT, 1, false>, a, NT, smem, dev, st);
+}
+
+int launch_row_grad(const char *who, RowGradArgs &a, int dtype, int mode, bool extra, int dev, cudaStream_t st) {
+  const int ne = a.n + (a.labels ? 1 : 0);
+  const size_t lists = (size_t)((ne + 3) & ~3) * 6 * 4;
+  const Plan p = plan_rows(a.in.logits, dtype, a.in.rows, a.in.V, a.in.ld, lists, device_sm_count(dev));
+  a.in.wps = p.wps;
+  a.in.C = p.C;
+  const size_t smem = (size_t)p.wps * 16 + lists;
+  return by_dtype(dtype, [&](auto e) {
+    using E = decltype(e);
+    return p.nt == 128 ? grad_nt<E, 128>(who, a, mode, extra, smem, dev, st)
+                       : grad_nt<E, 256>(who, a, mode, extra, smem, dev, st);
+  });
 }
 
 }  // namespace
@@ -447,11 +1276,30 @@ int launch_score(const char *who, const ScoreLaunch &s, cudaStream_t stream) {
                                   {"top_logprob", top ? s.top_logprob : nullptr}});
   if (dev < 0) return dev;
   DeviceGuard g(dev);
-  const ScoreArgs a{s.logits,  s.ld,    s.rows,      s.V,       s.tokens,   s.n_tok, (float)(1.0 / s.temperature),
-                    s.top_k,   s.logprob, s.entropy, s.top_ids, s.top_logprob};
-  const int grid = std::min(s.rows, 4 * device_sm_count(dev));
-  by_dtype(s.dtype, [&](auto e) { snai_score<decltype(e)><<<grid, kThreads, 0, stream>>>(a); });
-  return launched(who);
+  ScoreArgs a{};
+  a.in = Rows{s.logits, s.ld, s.rows, s.V, 0, 0};
+  a.tokens = s.tokens;
+  a.n_tok = s.n_tok;
+  a.c = (float)(1.4426950408889634 / s.temperature);
+  a.inv_t = (float)(1.0 / s.temperature);
+  a.top_k = s.top_k;
+  a.logprob = s.logprob;
+  a.entropy = s.entropy;
+  a.top_ids = s.top_ids;
+  a.top_logprob = s.top_logprob;
+  // room for half again the alternatives: the threshold lets a quarter more groups through
+  if (s.top_k)
+    for (a.cap = 128; a.cap < s.top_k + s.top_k / 2 + 64;) a.cap *= 2;
+  const size_t lists = s.top_k ? (size_t)(a.cap + s.top_k) * 8 : 0;
+  const Plan p = plan_rows(s.logits, s.dtype, s.rows, s.V, s.ld, lists + 18 * 1024, device_sm_count(dev));
+  a.in.wps = p.wps;
+  a.in.C = p.C;
+  const size_t maxima = ((size_t)((p.wps + kChunk * p.nt - 1) / (kChunk * p.nt)) + 1) * p.nt * 4;
+  const size_t smem = (size_t)p.wps * 16 + (s.top_k ? (size_t)(a.cap + (p.C > 1 ? s.top_k : 0)) * 8 + maxima : 0);
+  return by_dtype(s.dtype, [&](auto e) {
+    using E = decltype(e);
+    return p.nt == 128 ? score_nt<E, 128>(who, a, smem, dev, stream) : score_nt<E, 256>(who, a, smem, dev, stream);
+  });
 }
 
 int check_distill(const char *who, const DistillLaunch &s) {
@@ -496,15 +1344,22 @@ int launch_distill(const char *who, const DistillLaunch &s, cudaStream_t stream)
   if (dev < 0) return dev;
   DeviceGuard g(dev);
   RowGradArgs a{};
-  a.logits = s.logits, a.ld = s.ld, a.rows = s.rows, a.V = s.V;
-  a.ids = s.teacher_ids, a.n = s.top_k, a.vals = s.teacher_logits, a.labels = labels, a.row_grad = row_grad;
-  a.inv_td = 1.0 / s.temperature, a.inv_t = (float)a.inv_td;
-  a.t = (float)s.temperature, a.t2 = (float)(s.temperature * s.temperature);
-  a.a = (float)s.label_weight, a.rest = s.rest;
-  a.loss = s.loss, a.grad = s.grad, a.grad_ld = s.grad_ld;
-  const int grid = std::min(s.rows, 4 * device_sm_count(dev));
-  by_dtype(s.dtype, [&](auto e) { snai_row_grad<decltype(e), 1><<<grid, kThreads, 0, stream>>>(a); });
-  return launched(who);
+  a.in = Rows{s.logits, s.ld, s.rows, s.V, 0, 0};
+  a.ids = s.teacher_ids;
+  a.vals = s.teacher_logits;
+  a.n = s.top_k;
+  a.c = (float)(1.4426950408889634 / s.temperature);
+  a.inv_t = 1.0 / s.temperature;
+  a.inv_t_f = (float)a.inv_t;
+  a.labels = labels;
+  a.row_grad = row_grad;
+  a.t = s.temperature;
+  a.a = s.label_weight;
+  a.rest = s.rest;
+  a.loss = s.loss;
+  a.grad = s.grad;
+  a.grad_ld = s.grad_ld;
+  return launch_row_grad(who, a, s.dtype, 1, labels && s.temperature != 1.0, dev, stream);
 }
 
 }  // namespace snai
@@ -563,15 +1418,17 @@ extern "C" int cortex_score_grad(const void *logits, int dtype, int rows, int vo
   if (dev < 0) return dev;
   DeviceGuard g(dev);
   RowGradArgs a{};
-  a.logits = logits, a.ld = ld, a.rows = rows, a.V = vocab;
-  a.ids = tokens, a.n = n_tok, a.vals = g_logprob, a.g_entropy = g_entropy;
-  a.inv_td = 1.0 / temperature, a.inv_t = (float)a.inv_td;
-  a.grad = grad, a.grad_ld = grad_ld;
-  const int grid = std::min(rows, 4 * device_sm_count(dev));
-  by_dtype(dtype, [&](auto e) {
-    snai_row_grad<decltype(e), 0><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  });
-  return launched(who);
+  a.in = Rows{logits, ld, rows, vocab, 0, 0};
+  a.ids = tokens;
+  a.vals = g_logprob;
+  a.n = n_tok;
+  a.c = (float)(1.4426950408889634 / temperature);
+  a.inv_t = 1.0 / temperature;
+  a.inv_t_f = (float)a.inv_t;
+  a.g_entropy = g_entropy;
+  a.grad = grad;
+  a.grad_ld = grad_ld;
+  return launch_row_grad(who, a, dtype, 0, g_entropy != nullptr, dev, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int cortex_distill(const void *logits, int dtype, int rows, int vocab, long long ld,
