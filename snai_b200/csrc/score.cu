@@ -109,11 +109,11 @@ template <> struct Word<float> {
     unpack2(v[1], c, d);
     return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
   }
-  // maximum over kChunk words
-  __device__ static __forceinline__ float max(const uint4 *q) {
+  // maximum over N words
+  template <int N> __device__ static __forceinline__ float max(const uint4 *q) {
     float m = __uint_as_float(q[0].x);
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) {
+    for (int j = 0; j < N; ++j) {
       m = max_nan(m, max_nan(__uint_as_float(q[j].x), __uint_as_float(q[j].y)));
       m = max_nan(m, max_nan(__uint_as_float(q[j].z), __uint_as_float(q[j].w)));
     }
@@ -146,10 +146,10 @@ template <> struct Word<__nv_bfloat16> {
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
   }
-  __device__ static __forceinline__ float max(const uint4 *q) {
+  template <int N> __device__ static __forceinline__ float max(const uint4 *q) {
     unsigned m = q[0].x;
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) m = max2(m, max2(max2(q[j].x, q[j].y), max2(q[j].z, q[j].w)));
+    for (int j = 0; j < N; ++j) m = max2(m, max2(max2(q[j].x, q[j].y), max2(q[j].z, q[j].w)));
     return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
   }
   __device__ static __forceinline__ float one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
@@ -180,10 +180,10 @@ template <> struct Word<__half> {
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
   }
-  __device__ static __forceinline__ float max(const uint4 *q) {
+  template <int N> __device__ static __forceinline__ float max(const uint4 *q) {
     unsigned m = q[0].x;
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) m = max2(m, max2(max2(q[j].x, q[j].y), max2(q[j].z, q[j].w)));
+    for (int j = 0; j < N; ++j) m = max2(m, max2(max2(q[j].x, q[j].y), max2(q[j].z, q[j].w)));
     float a, b;
     unpack2(two(m), a, b);
     return max_nan(a, b);
@@ -216,52 +216,70 @@ struct Rows {
 
 // One CTA's slice of one row: words [first, first + n) of the row's 16-byte
 // grid, which starts `pad` elements before the row when the row does not
-// start on a word.  Thread t owns words t, t + NT, ... of the slice.
+// start on a word.  Thread t owns words t, t + NT, ... of the slice.  All
+// words are whole but the row's first and last, when they are ragged: whole
+// words are [lo, hi).
 template <typename E, int NT>
 struct Slice {
   static constexpr int kN = Word<E>::kN;
-  const E *row;  // the row's element 0
-  int pad, first, n, V;
+  static constexpr int kWide = kChunk * NT;  // words of a chunk over all threads
+  const char *src;  // the slice's word 0
+  int base;         // id of its element 0 (negative in the leading pad)
+  int n, lo, hi, V;
 
   __device__ __forceinline__ void set(const Rows &a, int r, unsigned rank) {
-    row = static_cast<const E *>(a.logits) + (long long)r * a.ld;
-    pad = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(E));
+    const char *row = static_cast<const char *>(a.logits) + (long long)r * a.ld * (int)sizeof(E);
+    const int pad = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(E));
+    const int first = (int)rank * a.wps, words = (pad + a.V + kN - 1) / kN;
     V = a.V;
-    first = (int)rank * a.wps;
-    n = min(a.wps, (pad + V + kN - 1) / kN - first);
+    base = first * kN - pad;
+    src = row + (long long)base * (int)sizeof(E);
+    n = min(a.wps, words - first);
+    lo = base < 0 ? 1 : 0;
+    hi = base + n * kN > V ? n - 1 : n;
   }
-  // id of element 0 of local word w (negative in the leading pad)
-  __device__ __forceinline__ int id0(int w) const { return (first + w) * kN - pad; }
-  __device__ __forceinline__ bool whole(int w) const {
-    const int i = id0(w);
-    return i >= 0 && i + kN <= V;
-  }
-  // local element index of an id, or -1 when another slice holds it
+  __device__ __forceinline__ int id0(int w) const { return base + w * kN; }
+  // local element index of an id, negative when another slice holds it
   __device__ __forceinline__ int local(int id) const {
-    const int e = id + pad - first * kN;
-    return e >= 0 && e < n * kN ? e : -1;
+    const int e = id - base;
+    return e < n * kN ? e : -1;
+  }
+  __device__ __forceinline__ const E *at(int id) const {
+    return reinterpret_cast<const E *>(src + (long long)(id - base) * (int)sizeof(E));
   }
   // Copies this thread's words of stage st (cps chunks) into buf and commits
   // them.  The row's ragged ends are filled up with -inf.
   __device__ __forceinline__ void load(int st, int cps, uint4 *buf) const {
-    for (int c = st * cps; c < (st + 1) * cps; ++c)
+    for (int c = st * cps; c < (st + 1) * cps; ++c) {
+      const int w0 = c * kWide;
+      if (w0 >= n) break;
+      const uint32_t dst = smem_u32(buf) + (w0 + threadIdx.x) * 16;
+      const char *p = src + (long long)(w0 + (int)threadIdx.x) * 16;
+      if (w0 >= lo && w0 + kWide <= hi) {
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) {
-        const int w = (c * kChunk + j) * NT + (int)threadIdx.x;
-        if (w >= n) break;
-        if (whole(w))
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(buf + w)), "l"(row + id0(w))
-                       : "memory");
-        else
-          ragged(w, buf);
+        for (int j = 0; j < kChunk; ++j) copy16(dst + j * NT * 16, p + j * NT * 16);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          const int w = w0 + j * NT + (int)threadIdx.x;
+          if (w >= lo && w < hi)
+            copy16(dst + j * NT * 16, p + j * NT * 16);
+          else if (w < n)
+            ragged(w, buf);
+        }
       }
+    }
     asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ static __forceinline__ void copy16(uint32_t dst, const char *p) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(p) : "memory");
   }
   __device__ __noinline__ void ragged(int w, uint4 *buf) const {
     E *p = reinterpret_cast<E *>(buf + w);
     const int i0 = id0(w);
-    for (int k = 0; k < kN; ++k) Word<E>::put(p + k, i0 + k >= 0 && i0 + k < V ? Word<E>::one(row + i0 + k) : -INFINITY);
+    for (int k = 0; k < kN; ++k) Word<E>::put(p + k, i0 + k >= 0 && i0 + k < V ? Word<E>::one(at(i0 + k)) : -INFINITY);
   }
+  // out: the output row's element 0
   __device__ __noinline__ void store_ragged(int w, uint4 q, E *out) const {
     const E *p = reinterpret_cast<const E *>(&q);
     const int i0 = id0(w);
@@ -270,11 +288,14 @@ struct Slice {
   }
   // this thread's four words of chunk c (all masked past the slice's end)
   __device__ __forceinline__ void chunk(int c, const uint4 *buf, uint4 *q) const {
+    const int w0 = c * kWide + (int)threadIdx.x;
+    if ((c + 1) * kWide <= n) {
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) {
-      const int w = (c * kChunk + j) * NT + (int)threadIdx.x;
-      const unsigned k = Word<E>::kMasked;
-      q[j] = w < n ? buf[w] : make_uint4(k, k, k, k);
+      for (int j = 0; j < kChunk; ++j) q[j] = buf[w0 + j * NT];
+    } else {
+      constexpr unsigned k = Word<E>::kMasked;
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) q[j] = w0 + j * NT < n ? buf[w0 + j * NT] : make_uint4(k, k, k, k);
     }
   }
 };
@@ -366,7 +387,7 @@ __device__ __forceinline__ Stat no_stat() { return {-FLT_MAX, 0.f, 0.f, 0.f}; }
 struct __align__(16) Slip {
   Stat st;
   double v[6];  // sums over the entries of a list (row gradients)
-  int count;    // alternatives in its list (scores)
+  float tau;    // a bound of its alternatives (scores)
 };
 
 __device__ __forceinline__ Stat peer_stat(const Slip *mine, unsigned rank) {
@@ -394,7 +415,9 @@ __device__ __forceinline__ float log_p(float z, float m, float inv_t, float s, f
 
 // The k-th largest of the groups' maxima (n values in shared memory), or a
 // little less, by one warp: at least k of the groups reach it, so at least k
-// elements do.  -inf when there are fewer groups than k.
+// elements do.  -inf when there are fewer groups than k.  N values a lane are
+// held in registers (N = 0: read again each time).
+template <int N>
 __device__ __forceinline__ float kth_of_maxima(const float *g, int n, int k) {
   if (n < k) return -INFINITY;
   const int lane = threadIdx.x & 31;
@@ -402,19 +425,32 @@ __device__ __forceinline__ float kth_of_maxima(const float *g, int n, int k) {
     const int b = __float_as_int(v);
     return b ^ ((b >> 31) & 0x7fffffff);
   };
+  int v[N ? N : 1];
   int lo = 0x7fffffff, hi = (int)0x80000000;
-  for (int i = lane; i < n; i += 32) {
-    const int v = ordered(g[i]);
-    lo = min(lo, v), hi = max(hi, v);
+  if (N) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = ordered(g[i * 32 + lane]);
+      lo = min(lo, v[i]), hi = max(hi, v[i]);
+    }
+  } else {
+    for (int i = lane; i < n; i += 32) {
+      const int x = ordered(g[i]);
+      lo = min(lo, x), hi = max(hi, x);
+    }
   }
-  lo = __reduce_min_sync(0xffffffffu, lo);
+  lo = __reduce_min_sync(0xffffffffu, lo);  // at least k groups reach lo
   hi = __reduce_max_sync(0xffffffffu, hi);
-  // at least k groups reach lo
   const int slack = k + (k >> 2) + 2;
   while (lo < hi) {
     const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) >> 1);
     int c = 0;
-    for (int i = lane; i < n; i += 32) c += ordered(g[i]) >= mid;
+    if (N) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) c += v[i] >= mid;
+    } else {
+      for (int i = lane; i < n; i += 32) c += ordered(g[i]) >= mid;
+    }
     c = __reduce_add_sync(0xffffffffu, c);
     if (c >= k) {
       lo = mid;
@@ -426,32 +462,42 @@ __device__ __forceinline__ float kth_of_maxima(const float *g, int n, int k) {
   return __int_as_float(lo ^ ((lo >> 31) & 0x7fffffff));
 }
 
+// Alternatives without sorting the row: each slice gives a value that at
+// least ceil(k / C) of its logits reach (from maxima kept in pass A), the
+// least of those over the C slices is reached by at least k logits of the
+// row, and usually by few more.  Those - the candidates - are collected in
+// one CTA of the cluster (each in turn, row by row), which orders them.
 template <typename E, int NT, bool TOPK, bool ENT>
 __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreArgs a) {
   constexpr int NW = NT / 32;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Stat part[2][NW];
   __shared__ Slip slip[2];
-  __shared__ float tau;
-  __shared__ int n_cand, n_ge;
+  __shared__ int counts[2];  // candidates collected; keys counted
   uint4 *buf = reinterpret_cast<uint4 *>(smem);
-  // alternatives: candidates, then (clusters) the slice's sorted list, the maxima of the chunks and of the threads
+  // candidates, then the maxima of the chunks and of the threads
   unsigned long long *cand = reinterpret_cast<unsigned long long *>(smem + (size_t)a.in.wps * 16);
-  unsigned long long *list = cand + a.cap;
-  float *cmax = reinterpret_cast<float *>(list + (a.in.C > 1 ? a.top_k : 0));
+  float *cmax = reinterpret_cast<float *>(cand + a.cap);
   const int t = threadIdx.x, lane = t & 31, wid = t >> 5;
   const int C = a.in.C;
   const unsigned rank = C > 1 ? cluster_ctarank() : 0;
   const int step = gridDim.x / C;
   const int chunks = (a.in.wps + kChunk * NT - 1) / (kChunk * NT), cps = (chunks + kStages - 1) / kStages;
   float *tmax = cmax + chunks * NT;
+  auto sync = [&] {
+    if (C > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+  };
 
   Slice<E, NT> cur, nxt;
   int r = blockIdx.x / C;
   cur.set(a.in, r, rank);
   for (int s = 0; s < kStages; ++s) cur.load(s, cps, buf);
   int par = 0;
-  for (; r < a.in.rows; r += step, par ^= 1) {
+  unsigned lead = 0;  // the CTA that orders this row's candidates
+  for (; r < a.in.rows; r += step, par ^= 1, lead = lead + 1 == (unsigned)C ? 0 : lead + 1) {
     const bool more = r + step < a.in.rows;
     if (more) nxt.set(a.in, r + step, rank);
     // the tokens' logits, read beside the row's copies
@@ -465,7 +511,7 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
         if (j < a.n_tok) {
           const int id = a.tokens[(long long)r * a.n_tok + j];
           in[i] = id >= 0 && id < a.in.V;
-          if (in[i]) zt[i] = Word<E>::one(cur.row + id);
+          if (in[i]) zt[i] = Word<E>::one(cur.at(id));
         }
       }
     // pass A
@@ -475,7 +521,7 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
       for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
         uint4 q[kChunk];
         cur.chunk(c, buf, q);
-        const float cm = Word<E>::max(q);
+        const float cm = Word<E>::template max<kChunk>(q);
         run.add(q, cm, a.c);
         if (TOPK) {
           cmax[c * NT + t] = cm;
@@ -499,27 +545,34 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
     Stat st = combine_lanes<ENT, false>(run.get(), 32, a.c);
     if (lane == 0) part[par][wid] = st;
     __syncthreads();
-    st = combine_lanes<ENT, false>(part[par][lane % NW], NW, a.c);
-    const bool bad_slice = st.s != st.s;
-    const int kl = TOPK ? max(0, min(a.top_k, min(cur.V, cur.id0(cur.n)) - max(0, cur.id0(0)))) : 0;
-    if (TOPK) {
-      // a lower bound of the slice's kl-th largest logit: from the threads'
-      // maxima when those are many more than kl, else from the chunks'
-      if (wid == 0) {
-        const bool few = 4 * kl <= NT;
-        const float b = bad_slice || kl == 0 ? INFINITY : kth_of_maxima(few ? tmax : cmax, few ? NT : chunks * NT, kl);
-        if (lane == 0) tau = b, n_cand = 0;
+    float tau = 0.f;
+    if (C > 1 || (TOPK && wid == 0)) {
+      st = combine_lanes<ENT, false>(part[par][lane % NW], NW, a.c);
+      if (TOPK && wid == 0) {
+        const int k = (a.top_k + C - 1) / C;
+        // the threads' maxima when those are many more than k, else the chunks'
+        tau = st.s != st.s     ? INFINITY
+              : 4 * k <= NT    ? kth_of_maxima<NT / 32>(tmax, NT, k)
+              : chunks == 4    ? kth_of_maxima<NT / 8>(cmax, 4 * NT, k)
+                               : kth_of_maxima<0>(cmax, chunks * NT, k);
       }
-      __syncthreads();
+      if (t == 0) slip[par].st = st, slip[par].tau = tau, counts[0] = 0;
     }
+    if (C > 1 || TOPK) sync();
     if (C > 1) {
-      if (t == 0) slip[par].st = st, slip[par].count = bad_slice ? 0 : kl;
-      cluster_sync_all();
-      st = combine_lanes<ENT, false>(lane % 16 < C ? peer_stat(&slip[par], lane % 16) : no_stat(), 16, a.c);
+      const bool on = lane % 16 < C;
+      st = combine_lanes<ENT, false>(on ? peer_stat(&slip[par], lane % 16) : no_stat(), 16, a.c);
+      if (TOPK) {
+        tau = on ? __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&slip[par].tau), lane % 16))) : INFINITY;
+        tau = -warp_max_nan(-tau);
+      }
+    } else {
+      st = combine_lanes<ENT, false>(part[par][lane % NW], NW, a.c);
+      if (TOPK) tau = slip[par].tau;
     }
-    const float ls = logf(st.s);
     const bool bad = st.s != st.s;
-    if (rank == 0) {
+    if (rank == 0 && t < max(a.n_tok, 1)) {
+      const float ls = logf(st.s);
 #pragma unroll
       for (int i = 0; i < kMaxList / NT; ++i) {
         const int j = i * NT + t;
@@ -529,16 +582,18 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
       if (ENT && t == 0 && a.entropy) a.entropy[r] = st.s == 0.f ? 0.f : ls - kLn2 * st.w / st.s;
     }
     if (TOPK) {
-      // candidates: this thread's elements that reach tau
-      const float b = tau;
-      auto each = [&](float least, auto f) {  // f(z, id) for own elements of chunks whose maximum reaches `least`
+      // f(z, id) for this thread's elements z >= least
+      auto each = [&](float least, auto f) {
         for (int c = 0; c < chunks; ++c) {
           if (!(cmax[c * NT + t] >= least)) continue;
           for (int j = 0; j < kChunk; ++j) {
             const int w = (c * kChunk + j) * NT + t;
             if (w >= cur.n) break;
+            const uint4 q = buf[w];
+            if (!(Word<E>::template max<1>(&q) >= least)) continue;
             const E *p = reinterpret_cast<const E *>(buf + w);
             const int i0 = cur.id0(w);
+#pragma unroll
             for (int k = 0; k < Word<E>::kN; ++k) {
               const float z = Word<E>::one(p + k);
               if (z >= least && i0 + k >= 0 && i0 + k < cur.V) f(z, i0 + k);
@@ -546,28 +601,43 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
           }
         }
       };
-      if (tm >= b)
-        each(b, [&](float z, int id) {
-          const int i = atomicAdd(&n_cand, 1);
+      const uint32_t lead_count = C > 1 ? mapa_shared(smem_u32(&counts[0]), lead) : 0;
+      const uint32_t lead_cand = C > 1 ? mapa_shared(smem_u32(cand), lead) : 0;
+      auto collect = [&](float z, int id) {
+        if (C > 1) {
+          const unsigned i = atom_cluster_add_u32(lead_count, 1);
+          if (i < (unsigned)a.cap) st_cluster_u64(lead_cand + 8 * i, sort_key(z, id));
+        } else {
+          const int i = atomicAdd(&counts[0], 1);
           if (i < a.cap) cand[i] = sort_key(z, id);
-        });
-      __syncthreads();
-      int n = n_cand;
+        }
+      };
+      auto count = [&](int i) {  // counts[i] of the leader
+        return C > 1 ? (int)ld_cluster_u32(mapa_shared(smem_u32(&counts[i]), lead)) : counts[i];
+      };
+      if (!bad && tm >= tau) each(tau, collect);
+      sync();
+      int n = count(0);
       if (n > a.cap) {
-        // too many (ties, few groups): bisect over whole keys to between kl and cap of them
-        unsigned long long lo = sort_key(b, INT_MAX), hi = ~0ull;
+        // too many (ties, few groups): bisect over whole keys to between k and cap of them
+        unsigned long long lo = sort_key(tau, INT_MAX), hi = ~0ull;
         for (;;) {
           const unsigned long long mid = lo + ((hi - lo) >> 1) + 1;
-          __syncthreads();
-          if (t == 0) n_ge = 0, n_cand = 0;
-          __syncthreads();
-          int cnt = 0;
-          each(key_logit(mid), [&](float z, int id) { cnt += sort_key(z, id) >= mid; });
-          cnt = __reduce_add_sync(0xffffffffu, cnt);
-          if (lane == 0) atomicAdd(&n_ge, cnt);
-          __syncthreads();
-          n = n_ge;
-          if (n < kl) {
+          sync();
+          if (t == 0) counts[0] = counts[1] = 0;
+          sync();
+          int c = 0;
+          each(key_logit(mid), [&](float z, int id) { c += sort_key(z, id) >= mid; });
+          c = __reduce_add_sync(0xffffffffu, c);
+          if (lane == 0 && c) {
+            if (C > 1)
+              atom_cluster_add_u32(mapa_shared(smem_u32(&counts[1]), lead), (unsigned)c);
+            else
+              atomicAdd(&counts[1], c);
+          }
+          sync();
+          n = count(1);
+          if (n < a.top_k) {
             hi = mid - 1;
           } else {
             lo = mid;
@@ -575,77 +645,59 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
           }
         }
         each(key_logit(lo), [&](float z, int id) {
-          const unsigned long long k = sort_key(z, id);
-          if (k >= lo) cand[atomicAdd(&n_cand, 1)] = k;
+          if (sort_key(z, id) >= lo) collect(z, id);
         });
-        __syncthreads();
+        sync();
       }
       if (more)
         for (int s = 0; s < kStages; ++s) nxt.load(s, cps, buf);
-      // order them: by counting when they are few, else a bitonic sort
-      auto place = [&](int at, unsigned long long key) {
-        if (C > 1) {
-          list[at] = key;
+      if (rank == lead) {
+        // order them: by counting when they are few, else a bitonic sort
+        int *ids = a.top_ids + (long long)r * a.top_k;
+        float *lps = a.top_logprob + (long long)r * a.top_k;
+        const float ls = logf(st.s);
+        if (bad) {
+          for (int i = t; i < a.top_k; i += NT) ids[i] = -1, lps[i] = NAN;
+        } else if (n <= 192) {
+          for (int i = t; i < n; i += NT) {
+            const unsigned long long key = cand[i];
+            int above = 0;
+#pragma unroll 4
+            for (int j = 0; j + 1 < n; j += 2) {
+              const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(cand + j);
+              above += (v.x > key) + (v.y > key);
+            }
+            if (n & 1) above += cand[n - 1] > key;
+            if (above < a.top_k) {
+              ids[above] = key_id(key);
+              lps[above] = log_p(key_logit(key), st.m, a.inv_t, st.s, ls);
+            }
+          }
         } else {
-          a.top_ids[(long long)r * a.top_k + at] = key_id(key);
-          a.top_logprob[(long long)r * a.top_k + at] = log_p(key_logit(key), st.m, a.inv_t, st.s, ls);
-        }
-      };
-      if (n <= 192) {
-        for (int i = t; i < n; i += NT) {
-          const unsigned long long key = cand[i];
-          int above = 0;
-          for (int j = 0; j < n; ++j) above += cand[j] > key;
-          if (above < kl) place(above, key);
-        }
-      } else {
-        int len = 256;
-        while (len < n) len *= 2;
-        for (int i = n + t; i < len; i += NT) cand[i] = 0;
-        for (int size = 2; size <= len; size *= 2)
-          for (int stride = size / 2; stride > 0; stride /= 2) {
-            __syncthreads();
-            for (int i = t; i < len / 2; i += NT) {
-              const int x = 2 * i - (i & (stride - 1)), y = x + stride;
-              const unsigned long long u = cand[x], v = cand[y];
-              if ((u < v) == ((x & size) == 0)) cand[x] = v, cand[y] = u;
+          int len = 256;
+          while (len < n) len *= 2;
+          for (int i = n + t; i < len; i += NT) cand[i] = 0;
+          for (int size = 2; size <= len; size *= 2)
+            for (int stride = size / 2; stride > 0; stride /= 2) {
+              __syncthreads();
+              for (int i = t; i < len / 2; i += NT) {
+                const int x = 2 * i - (i & (stride - 1)), y = x + stride;
+                const unsigned long long u = cand[x], v = cand[y];
+                if ((u < v) == ((x & size) == 0)) cand[x] = v, cand[y] = u;
+              }
             }
-          }
-        __syncthreads();
-        for (int i = t; i < kl; i += NT) place(i, cand[i]);
-      }
-      if (C > 1) {
-        // an entry's place among all slices: its own plus the greater ones of every other list
-        cluster_sync_all();
-        for (int i = t; i < (bad ? 0 : kl); i += NT) {
-          const unsigned long long key = list[i];
-          int at = i;
-          for (int o = 1; o < C; ++o) {
-            const unsigned peer = (rank + o) % C;
-            const uint32_t pl = mapa_shared(smem_u32(list), peer);
-            int x = 0, y = (int)ld_cluster_u32(mapa_shared(smem_u32(&slip[par].count), peer));
-            while (x < y) {
-              const int h = (x + y) / 2;
-              if (ld_cluster_u64(pl + 8 * h) > key)
-                x = h + 1;
-              else
-                y = h;
-            }
-            at += x;
-          }
-          if (at < a.top_k) {
-            a.top_ids[(long long)r * a.top_k + at] = key_id(key);
-            a.top_logprob[(long long)r * a.top_k + at] = log_p(key_logit(key), st.m, a.inv_t, st.s, ls);
+          __syncthreads();
+          for (int i = t; i < a.top_k; i += NT) {
+            const unsigned long long key = cand[i];
+            ids[i] = key_id(key);
+            lps[i] = log_p(key_logit(key), st.m, a.inv_t, st.s, ls);
           }
         }
       }
-      if (bad && rank == 0)
-        for (int i = t; i < a.top_k; i += NT)
-          a.top_ids[(long long)r * a.top_k + i] = -1, a.top_logprob[(long long)r * a.top_k + i] = NAN;
     }
     cur = nxt;
   }
-  if (C > 1) cluster_sync_all();  // others may still read this CTA's slip and list
+  if (C > 1) cluster_sync_all();  // others may still read this CTA's slip
 }
 
 // ---- row gradients ----
@@ -801,7 +853,7 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_row_grad(const Row
       for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
         uint4 q[kChunk];
         cur.chunk(c, buf, q);
-        run.add(q, Word<E>::max(q), a.c);
+        run.add(q, Word<E>::template max<kChunk>(q), a.c);
       }
     };
     copies_wait<3>(), stage(0);
@@ -946,7 +998,7 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_row_grad(const Row
     }
     // pass B
     E *out = static_cast<E *>(a.grad) + (long long)r * a.grad_ld;
-    const bool vec = ((reinterpret_cast<uintptr_t>(out) - cur.pad * sizeof(E)) & 15) == 0;
+    const bool vec = ((reinterpret_cast<uintptr_t>(out) + (long long)cur.base * (int)sizeof(E)) & 15) == 0;
     const f2 nm2 = pack2(-st.m, -st.m), c2 = pack2(a.c, a.c), l2 = pack2(kLog2E, kLog2E);
     const f2 al2 = pack2(alpha, alpha), be2 = pack2(beta, beta), ga2 = pack2(gamma, gamma);
 #pragma unroll 1
@@ -977,14 +1029,18 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_row_grad(const Row
           }
           q[j] = any ? Word<E>::pack(v) : make_uint4(0u, 0u, 0u, 0u);
         }
+        const int w0 = c * cur.kWide + t;
+        E *o = out + cur.id0(w0);
+        if (vec && c * cur.kWide >= cur.lo && (c + 1) * cur.kWide <= cur.hi) {
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-          const int w = (c * kChunk + j) * NT + t;
-          if (w < cur.n) {
-            const int i0 = cur.id0(w);
-            if (vec && cur.whole(w))
-              *reinterpret_cast<uint4 *>(out + i0) = q[j];
-            else
+          for (int j = 0; j < kChunk; ++j) *reinterpret_cast<uint4 *>(o + j * NT * kN) = q[j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) {
+            const int w = w0 + j * NT;
+            if (vec && w >= cur.lo && w < cur.hi)
+              *reinterpret_cast<uint4 *>(o + j * NT * kN) = q[j];
+            else if (w < cur.n)
               cur.store_ragged(w, q[j], out);
           }
         }
@@ -1290,12 +1346,12 @@ int launch_score(const char *who, const ScoreLaunch &s, cudaStream_t stream) {
   // room for half again the alternatives: the threshold lets a quarter more groups through
   if (s.top_k)
     for (a.cap = 128; a.cap < s.top_k + s.top_k / 2 + 64;) a.cap *= 2;
-  const size_t lists = s.top_k ? (size_t)(a.cap + s.top_k) * 8 : 0;
+  const size_t lists = s.top_k ? (size_t)a.cap * 8 : 0;
   const Plan p = plan_rows(s.logits, s.dtype, s.rows, s.V, s.ld, lists + 18 * 1024, device_sm_count(dev));
   a.in.wps = p.wps;
   a.in.C = p.C;
   const size_t maxima = ((size_t)((p.wps + kChunk * p.nt - 1) / (kChunk * p.nt)) + 1) * p.nt * 4;
-  const size_t smem = (size_t)p.wps * 16 + (s.top_k ? (size_t)(a.cap + (p.C > 1 ? s.top_k : 0)) * 8 + maxima : 0);
+  const size_t smem = (size_t)p.wps * 16 + (s.top_k ? lists + maxima : 0);
   return by_dtype(s.dtype, [&](auto e) {
     using E = decltype(e);
     return p.nt == 128 ? score_nt<E, 128>(who, a, smem, dev, stream) : score_nt<E, 256>(who, a, smem, dev, stream);
