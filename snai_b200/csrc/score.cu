@@ -41,6 +41,7 @@ constexpr int kMaxList = kScoreMaxK;
 constexpr int kMaxVocab = 1 << 19;  // as cortex_sample
 constexpr int kStages = 4;          // copy groups a row's words are committed in
 constexpr int kChunk = 4;           // words a thread takes at a time
+constexpr int kMaxCap = 2048;       // candidates of alternatives held at most
 constexpr float kLowest = -200.f;   // exponents (base 2) are cut here: 2^-200 is 0 in fp32, and 0 * d stays 0
 constexpr float kLn2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
 
@@ -210,8 +211,9 @@ struct Rows {
   const void *logits;
   long long ld;
   int rows, V;
-  int wps;  // words of a slice
-  int C;    // CTAs of a cluster, one slice each
+  int wps;    // words of a slice
+  int C;      // CTAs of a cluster, one slice each
+  bool even;  // all rows start at the same place of a 16-byte word
 };
 
 // One CTA's slice of one row: words [first, first + n) of the row's 16-byte
@@ -238,6 +240,13 @@ struct Slice {
     lo = base < 0 ? 1 : 0;
     hi = base + n * kN > V ? n - 1 : n;
   }
+  // the slice of row r + step
+  __device__ __forceinline__ void next(const Rows &a, int r, int step, unsigned rank) {
+    if (a.even)
+      src += (long long)step * a.ld * (int)sizeof(E);
+    else
+      set(a, r + step, rank);
+  }
   __device__ __forceinline__ int id0(int w) const { return base + w * kN; }
   // local element index of an id, negative when another slice holds it
   __device__ __forceinline__ int local(int id) const {
@@ -247,35 +256,37 @@ struct Slice {
   __device__ __forceinline__ const E *at(int id) const {
     return reinterpret_cast<const E *>(src + (long long)(id - base) * (int)sizeof(E));
   }
-  // Copies this thread's words of stage st (cps chunks) into buf and commits
-  // them.  The row's ragged ends are filled up with -inf.
-  __device__ __forceinline__ void load(int st, int cps, uint4 *buf) const {
-    for (int c = st * cps; c < (st + 1) * cps; ++c) {
-      const int w0 = c * kWide;
-      if (w0 >= n) break;
-      const uint32_t dst = smem_u32(buf) + (w0 + threadIdx.x) * 16;
-      const char *p = src + (long long)(w0 + (int)threadIdx.x) * 16;
-      if (w0 >= lo && w0 + kWide <= hi) {
+  // Copies this thread's words of chunk c to `to` (a chunk's place in shared
+  // memory).  The row's ragged ends are filled up with -inf.
+  __device__ __forceinline__ void load_chunk(int c, uint4 *to) const {
+    const int w0 = c * kWide;
+    const uint32_t dst = smem_u32(to + threadIdx.x);
+    const char *p = src + (long long)(w0 + (int)threadIdx.x) * 16;
+    if (w0 >= lo && w0 + kWide <= hi) {
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) copy16(dst + j * NT * 16, p + j * NT * 16);
-      } else {
+      for (int j = 0; j < kChunk; ++j) copy16(dst + j * NT * 16, p + j * NT * 16);
+    } else {
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-          const int w = w0 + j * NT + (int)threadIdx.x;
-          if (w >= lo && w < hi)
-            copy16(dst + j * NT * 16, p + j * NT * 16);
-          else if (w < n)
-            ragged(w, buf);
-        }
+      for (int j = 0; j < kChunk; ++j) {
+        const int w = w0 + j * NT + (int)threadIdx.x;
+        if (w >= lo && w < hi)
+          copy16(dst + j * NT * 16, p + j * NT * 16);
+        else if (w < n)
+          ragged(w, to + (w - w0));
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   }
+  // the words of stage st (cps chunks) of a row staged as a whole, committed as one group
+  __device__ __forceinline__ void load(int st, int cps, uint4 *buf) const {
+    for (int c = st * cps; c < (st + 1) * cps && c * kWide < n; ++c) load_chunk(c, buf + c * kWide);
+    commit();
+  }
+  __device__ static __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
   __device__ static __forceinline__ void copy16(uint32_t dst, const char *p) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(p) : "memory");
   }
-  __device__ __noinline__ void ragged(int w, uint4 *buf) const {
-    E *p = reinterpret_cast<E *>(buf + w);
+  __device__ __noinline__ void ragged(int w, uint4 *to) const {
+    E *p = reinterpret_cast<E *>(to);
     const int i0 = id0(w);
     for (int k = 0; k < kN; ++k) Word<E>::put(p + k, i0 + k >= 0 && i0 + k < V ? Word<E>::one(at(i0 + k)) : -INFINITY);
   }
@@ -286,16 +297,17 @@ struct Slice {
     for (int k = 0; k < kN; ++k)
       if (i0 + k >= 0 && i0 + k < V) out[i0 + k] = p[k];
   }
-  // this thread's four words of chunk c (all masked past the slice's end)
-  __device__ __forceinline__ void chunk(int c, const uint4 *buf, uint4 *q) const {
-    const int w0 = c * kWide + (int)threadIdx.x;
+  // this thread's four words of chunk c, staged at `at` (all masked past the slice's end)
+  __device__ __forceinline__ void chunk(int c, const uint4 *at, uint4 *q) const {
+    at += threadIdx.x;
     if ((c + 1) * kWide <= n) {
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) q[j] = buf[w0 + j * NT];
+      for (int j = 0; j < kChunk; ++j) q[j] = at[j * NT];
     } else {
       constexpr unsigned k = Word<E>::kMasked;
+      const int left = n - c * kWide - (int)threadIdx.x;
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) q[j] = w0 + j * NT < n ? buf[w0 + j * NT] : make_uint4(k, k, k, k);
+      for (int j = 0; j < kChunk; ++j) q[j] = j * NT < left ? at[j * NT] : make_uint4(k, k, k, k);
     }
   }
 };
@@ -324,13 +336,18 @@ __device__ __forceinline__ void rebase(Stat &a, float m, float c) {
   a.m = m;
 }
 
+// A thread's statistics as its words come.  m need not be the maximum: sums
+// relative to a value up to 2^kAbove below it are as good (a sum of 2^19 terms
+// stays far from fp32's end), so they are rebased only when a chunk's maximum
+// cm passes that: once or twice a row instead of at most chunks.
+constexpr float kAbove = 16.f;
 template <typename E, bool W, bool S1>
 struct Running {
-  float m = -FLT_MAX;
+  float m = -FLT_MAX, most = -FLT_MAX;
   f2 s = 0, w = 0, s1 = 0;
 
-  __device__ __forceinline__ void add(const uint4 *q, float cm, float c) {
-    if (!(cm <= m)) {  // a new maximum, or a NaN
+  __device__ __forceinline__ void add(const uint4 *q, float cm, float c, float above) {
+    if (!(cm <= most)) {  // far above, or a NaN
       const float nm = max_nan(m, cm), x = cut((m - nm) * c), f = ex2(x);
       const f2 ff = pack2(f, f);
       if (W) w = mul2(ff, fma2(s, pack2(x, x), w));
@@ -340,6 +357,7 @@ struct Running {
         s1 = mul2(pack2(f1, f1), s1);
       }
       m = nm;
+      most = nm + above;
     }
     const f2 nm2 = pack2(-m, -m), c2 = pack2(c, c), l2 = pack2(kLog2E, kLog2E);
 #pragma unroll
@@ -403,7 +421,7 @@ struct ScoreArgs {
   const int *tokens;
   int n_tok;
   float c, inv_t;  // log2(e) / T, 1 / T
-  int top_k, cap;  // cap: candidates the buffer holds (a power of two)
+  int top_k, cap, soft;  // candidates: what the buffer holds (a power of two), and where it is thinned out
   float *logprob, *entropy;
   int *top_ids;
   float *top_logprob;
@@ -413,12 +431,11 @@ __device__ __forceinline__ float log_p(float z, float m, float inv_t, float s, f
   return s == 0.f || z == -INFINITY ? -INFINITY + (s - s) : (z - m) * inv_t - ls;
 }
 
-// The k-th largest of the groups' maxima (n values in shared memory), or a
-// little less, by one warp: at least k of the groups reach it, so at least k
-// elements do.  -inf when there are fewer groups than k.  N values a lane are
-// held in registers (N = 0: read again each time).
-template <int N>
-__device__ __forceinline__ float kth_of_maxima(const float *g, int n, int k) {
+// A value that at least k of n values reach and few more do, by one warp:
+// their k-th largest, or a little less.  -inf when n < k.  at(i) is the i-th
+// value; N values a lane are held in registers (N = 0: fetched each time).
+template <int N, class At>
+__device__ __forceinline__ float about_kth(At at, int n, int k) {
   if (n < k) return -INFINITY;
   const int lane = threadIdx.x & 31;
   auto ordered = [](float v) {
@@ -430,16 +447,17 @@ __device__ __forceinline__ float kth_of_maxima(const float *g, int n, int k) {
   if (N) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      v[i] = ordered(g[i * 32 + lane]);
-      lo = min(lo, v[i]), hi = max(hi, v[i]);
+      v[i] = ordered(i * 32 + lane < n ? at(i * 32 + lane) : -INFINITY);
+      if (i * 32 + lane < n) lo = min(lo, v[i]);
+      hi = max(hi, v[i]);
     }
   } else {
     for (int i = lane; i < n; i += 32) {
-      const int x = ordered(g[i]);
+      const int x = ordered(at(i));
       lo = min(lo, x), hi = max(hi, x);
     }
   }
-  lo = __reduce_min_sync(0xffffffffu, lo);  // at least k groups reach lo
+  lo = __reduce_min_sync(0xffffffffu, lo);  // k values reach lo
   hi = __reduce_max_sync(0xffffffffu, hi);
   const int slack = k + (k >> 2) + 2;
   while (lo < hi) {
@@ -449,7 +467,7 @@ __device__ __forceinline__ float kth_of_maxima(const float *g, int n, int k) {
 #pragma unroll
       for (int i = 0; i < N; ++i) c += v[i] >= mid;
     } else {
-      for (int i = lane; i < n; i += 32) c += ordered(g[i]) >= mid;
+      for (int i = lane; i < n; i += 32) c += ordered(at(i)) >= mid;
     }
     c = __reduce_add_sync(0xffffffffu, c);
     if (c >= k) {
@@ -462,44 +480,104 @@ __device__ __forceinline__ float kth_of_maxima(const float *g, int n, int k) {
   return __int_as_float(lo ^ ((lo >> 31) & 0x7fffffff));
 }
 
-// Alternatives without sorting the row: each slice gives a value that at
-// least ceil(k / C) of its logits reach (from maxima kept in pass A), the
-// least of those over the C slices is reached by at least k logits of the
-// row, and usually by few more.  Those - the candidates - are collected in
-// one CTA of the cluster (each in turn, row by row), which orders them.
-template <typename E, int NT, bool TOPK, bool ENT>
+// Writes the k greatest of n keys (k <= n; ids and log p, in order): by
+// counting the greater ones when they are few, else by a bitonic sort (cand
+// holds a power of two of at least n keys).  The whole block calls it.
+template <int NT>
+__device__ __forceinline__ void put_greatest(unsigned long long *cand, int n, int k, int *ids, float *lps, float m,
+                                             float inv_t, float s) {
+  const int t = threadIdx.x;
+  const float ls = logf(s);
+  auto put = [&](int i, unsigned long long key) {
+    ids[i] = key_id(key);
+    lps[i] = log_p(key_logit(key), m, inv_t, s, ls);
+  };
+  if (n <= 256) {
+    for (int i = t; i < n; i += NT) {
+      const unsigned long long key = cand[i];
+      int above = 0;
+#pragma unroll 4
+      for (int j = 0; j + 1 < n; j += 2) {
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(cand + j);
+        above += (v.x > key) + (v.y > key);
+      }
+      if (n & 1) above += cand[n - 1] > key;
+      if (above < k) put(above, key);
+    }
+    return;
+  }
+  int len = 512;
+  while (len < n) len *= 2;
+  for (int i = n + t; i < len; i += NT) cand[i] = 0;
+  for (int size = 2; size <= len; size *= 2)
+    for (int stride = size / 2; stride > 0; stride /= 2) {
+      __syncthreads();
+      for (int i = t; i < len / 2; i += NT) {
+        const int x = 2 * i - (i & (stride - 1)), y = x + stride;
+        const unsigned long long u = cand[x], v = cand[y];
+        if ((u < v) == ((x & size) == 0)) cand[x] = v, cand[y] = u;
+      }
+    }
+  __syncthreads();
+  for (int i = t; i < k; i += NT) put(i, cand[i]);
+}
+
+// Rows stream through a ring of D chunks of shared memory: a thread waits for
+// its own words, takes them up, and sends for the chunk D further on, of this
+// row or the next.
+//
+// Alternatives are found on the way, in one reading.  From the first chunk's
+// maxima (of each thread's words, or of each word when k is large) comes a
+// value tau that at least k logits reach; what reaches it is a candidate.  In
+// later chunks only logits above tau can be alternatives, since equal ones
+// have greater ids than k others.  When the candidates pass a soft limit tau
+// is raised to about their k-th greatest and the rest dropped; a chunk that
+// brings more than the buffer holds (rows of equal or ascending logits) is
+// cut exactly, by bisection over (logit, id) keys.  What remains is ordered
+// at the row's end.
+//
+// A row over a cluster (few rows) has each slice find its own candidates;
+// those that reach the least of the slices' about ceil(k / C)-th greatest are
+// at least k, and go to rank 0, which orders them.
+template <typename E, int NT, int D, bool TOPK, bool ENT>
 __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreArgs a) {
-  constexpr int NW = NT / 32;
+  constexpr int NW = NT / 32, kWide = kChunk * NT, kN = Word<E>::kN;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Stat part[2][NW];
   __shared__ Slip slip[2];
-  __shared__ int counts[2];  // candidates collected; keys counted
-  uint4 *buf = reinterpret_cast<uint4 *>(smem);
-  // candidates, then the maxima of the chunks and of the threads
-  unsigned long long *cand = reinterpret_cast<unsigned long long *>(smem + (size_t)a.in.wps * 16);
-  float *cmax = reinterpret_cast<float *>(cand + a.cap);
+  __shared__ float tau_s;
+  __shared__ int n_cand, n_ge, n_lead;
+  uint4 *ring = reinterpret_cast<uint4 *>(smem);
+  // candidates, then (rank 0 of a cluster) those of all slices, then the first chunk's maxima
+  unsigned long long *cand = reinterpret_cast<unsigned long long *>(smem + D * kWide * 16);
+  unsigned long long *gath = cand + a.cap;
+  float *maxima = reinterpret_cast<float *>(gath + (a.in.C > 1 ? a.cap : 0));
   const int t = threadIdx.x, lane = t & 31, wid = t >> 5;
   const int C = a.in.C;
   const unsigned rank = C > 1 ? cluster_ctarank() : 0;
   const int step = gridDim.x / C;
-  const int chunks = (a.in.wps + kChunk * NT - 1) / (kChunk * NT), cps = (chunks + kStages - 1) / kStages;
-  float *tmax = cmax + chunks * NT;
-  auto sync = [&] {
-    if (C > 1)
-      cluster_sync_all();
-    else
-      __syncthreads();
-  };
+  const int chunks = (a.in.wps + kWide - 1) / kWide;
+  const float above = kAbove / a.c;
+  const bool by_word = 4 * a.top_k > NT;
 
-  Slice<E, NT> cur, nxt;
-  int r = blockIdx.x / C;
+  Slice<E, NT> cur, ahead;  // the row in work, the row being sent for
+  int r = blockIdx.x / C, ra = r, ca = 0, slot = 0;
   cur.set(a.in, r, rank);
-  for (int s = 0; s < kStages; ++s) cur.load(s, cps, buf);
+  ahead = cur;
+  auto send = [&](uint4 *to) {  // the next chunk of the stream, a group of its own
+    if (ra < a.in.rows) {
+      ahead.load_chunk(ca, to);
+      if (++ca == chunks) {
+        ca = 0;
+        if (ra + step < a.in.rows) ahead.next(a.in, ra, step, rank);
+        ra += step;
+      }
+    }
+    ahead.commit();
+  };
+  for (int i = 0; i < D; ++i) send(ring + i * kWide);
   int par = 0;
-  unsigned lead = 0;  // the CTA that orders this row's candidates
-  for (; r < a.in.rows; r += step, par ^= 1, lead = lead + 1 == (unsigned)C ? 0 : lead + 1) {
-    const bool more = r + step < a.in.rows;
-    if (more) nxt.set(a.in, r + step, rank);
+  for (; r < a.in.rows; par ^= 1) {
     // the tokens' logits, read beside the row's copies
     float zt[kMaxList / NT];
     bool in[kMaxList / NT];
@@ -514,63 +592,153 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
           if (in[i]) zt[i] = Word<E>::one(cur.at(id));
         }
       }
-    // pass A
     Running<E, ENT, false> run;
-    float tm = -INFINITY;
-    auto stage = [&](int s) {
-      for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
-        uint4 q[kChunk];
-        cur.chunk(c, buf, q);
-        const float cm = Word<E>::template max<kChunk>(q);
-        run.add(q, cm, a.c);
-        if (TOPK) {
-          cmax[c * NT + t] = cm;
-          tm = max_nan(tm, cm);
+    float tau = -INFINITY;
+    for (int c = 0; c < chunks; ++c) {
+      uint4 *at = ring + slot * kWide;
+      slot = slot + 1 == D ? 0 : slot + 1;
+      copies_wait<D - 1>();
+      uint4 q[kChunk];
+      cur.chunk(c, at, q);
+      const float cm = Word<E>::template max<kChunk>(q);
+      run.add(q, cm, a.c, above);
+      if (TOPK) {
+        const int w0 = c * kWide + t;
+        // f(z, id) for this thread's logits of the chunk that reach `least`
+        auto each = [&](float least, auto f) {
+          for (int j = 0; j < kChunk; ++j) {
+            if (w0 + j * NT >= cur.n) break;
+            const uint4 w = at[j * NT + t];
+            if (!(Word<E>::template max<1>(&w) >= least)) continue;
+            const E *p = reinterpret_cast<const E *>(at + j * NT + t);
+            const int i0 = cur.id0(w0 + j * NT);
+            for (int k = 0; k < kN; ++k) {
+              const float z = Word<E>::one(p + k);
+              if (z >= least && i0 + k >= 0 && i0 + k < cur.V) f(z, i0 + k);
+            }
+          }
+        };
+        int last = -1;  // this thread's last place in the buffer
+        auto push = [&](unsigned long long key) {
+          last = atomicAdd(&n_cand, 1);
+          if (last < a.cap) cand[last] = key;
+        };
+        bool full;
+        if (c == 0) {
+          if (by_word) {
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) maxima[j * NT + t] = Word<E>::template max<1>(q + j);
+          } else {
+            maxima[t] = cm;
+          }
+          __syncthreads();
+          if (wid == 0) {
+            auto val = [&](int i) { return maxima[i]; };
+            const float b = by_word ? about_kth<0>(val, kChunk * NT, a.top_k) : about_kth<NT / 32>(val, NT, a.top_k);
+            if (lane == 0) tau_s = b, n_cand = 0;
+          }
+          __syncthreads();
+          tau = tau_s;
+          if (cm >= tau) each(tau, [&](float z, int id) { push(sort_key(z, id)); });
+        } else if (cm > tau) {
+          each(tau, [&](float z, int id) {
+            if (z > tau) push(sort_key(z, id));
+          });
+        }
+        full = __syncthreads_or(last >= a.soft);
+        if (full) {
+          const int n = n_cand;
+          __syncthreads();
+          if (n <= a.cap) {
+            // drop what cannot be among the k greatest
+            if (wid == 0) {
+              const float b = about_kth<0>([&](int i) { return key_logit(cand[i]); }, n, a.top_k);
+              if (lane == 0) tau_s = b, n_cand = 0;
+            }
+            __syncthreads();
+            tau = tau_s;
+            unsigned long long own[kMaxCap / NT];
+            int m = 0;
+#pragma unroll
+            for (int i = 0; i < kMaxCap / NT; ++i) {
+              own[i] = i * NT + t < n ? cand[i * NT + t] : 0;
+              if (i * NT + t < n && key_logit(own[i]) >= tau)
+                ++m;
+              else
+                own[i] = 0;
+            }
+            __syncthreads();
+            int p = m ? atomicAdd(&n_cand, m) : 0;
+#pragma unroll
+            for (int i = 0; i < kMaxCap / NT; ++i)
+              if (own[i]) cand[p++] = own[i];
+            __syncthreads();
+          } else {
+            // more than the buffer holds: the candidates of earlier chunks
+            // and all of this one, cut to between k and cap
+            const int floor_id = c == 0 ? 0 : cur.id0(c * kWide);
+            unsigned long long lo = sort_key(tau, INT_MAX), hi = ~0ull;
+            auto old = [&](int i) { return key_id(cand[i]) < floor_id ? cand[i] : 0ull; };
+            for (;;) {
+              const unsigned long long mid = lo + ((hi - lo) >> 1) + 1;
+              __syncthreads();
+              if (t == 0) n_ge = 0;
+              __syncthreads();
+              int g = 0;
+              for (int i = t; i < a.cap; i += NT) g += old(i) >= mid;
+              each(key_logit(mid), [&](float z, int id) { g += sort_key(z, id) >= mid; });
+              g = __reduce_add_sync(0xffffffffu, g);
+              if (lane == 0 && g) atomicAdd(&n_ge, g);
+              __syncthreads();
+              g = n_ge;
+              if (g < a.top_k) {
+                hi = mid - 1;
+              } else {
+                lo = mid;
+                if (g <= a.soft) break;
+              }
+            }
+            unsigned long long own[kMaxCap / NT];
+#pragma unroll
+            for (int i = 0; i < kMaxCap / NT; ++i) own[i] = i * NT + t < a.cap ? old(i * NT + t) : 0;
+            __syncthreads();
+            if (t == 0) n_cand = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kMaxCap / NT; ++i)
+              if (own[i] >= lo) push(own[i]);
+            each(key_logit(lo), [&](float z, int id) {
+              if (sort_key(z, id) >= lo) push(sort_key(z, id));
+            });
+            tau = key_logit(lo);
+            __syncthreads();
+          }
         }
       }
-      if (!TOPK && more) nxt.load(s, cps, buf);
-    };
-    if (!TOPK && more) {  // one group of the next row follows each stage
-      copies_wait<kStages - 1>(), stage(0);
-      copies_wait<kStages - 1>(), stage(1);
-      copies_wait<kStages - 1>(), stage(2);
-      copies_wait<kStages - 1>(), stage(3);
-    } else {
-      copies_wait<3>(), stage(0);
-      copies_wait<2>(), stage(1);
-      copies_wait<1>(), stage(2);
-      copies_wait<0>(), stage(3);
+      send(at);
     }
-    if (TOPK) tmax[t] = tm;
     Stat st = combine_lanes<ENT, false>(run.get(), 32, a.c);
     if (lane == 0) part[par][wid] = st;
     __syncthreads();
-    float tau = 0.f;
-    if (C > 1 || (TOPK && wid == 0)) {
-      st = combine_lanes<ENT, false>(part[par][lane % NW], NW, a.c);
-      if (TOPK && wid == 0) {
-        const int k = (a.top_k + C - 1) / C;
-        // the threads' maxima when those are many more than k, else the chunks'
-        tau = st.s != st.s     ? INFINITY
-              : 4 * k <= NT    ? kth_of_maxima<NT / 32>(tmax, NT, k)
-              : chunks == 4    ? kth_of_maxima<NT / 8>(cmax, 4 * NT, k)
-                               : kth_of_maxima<0>(cmax, chunks * NT, k);
-      }
-      if (t == 0) slip[par].st = st, slip[par].tau = tau, counts[0] = 0;
-    }
-    if (C > 1 || TOPK) sync();
+    const int n = TOPK ? n_cand : 0;
     if (C > 1) {
+      if (wid == 0) {
+        st = combine_lanes<ENT, false>(part[par][lane % NW], NW, a.c);
+        if (TOPK)
+          tau = st.s != st.s ? INFINITY
+                             : about_kth<0>([&](int i) { return key_logit(cand[i]); }, n, (a.top_k + C - 1) / C);
+        if (lane == 0) slip[par].st = st, slip[par].tau = tau, n_lead = 0;
+      }
+      cluster_sync_all();
       const bool on = lane % 16 < C;
       st = combine_lanes<ENT, false>(on ? peer_stat(&slip[par], lane % 16) : no_stat(), 16, a.c);
       if (TOPK) {
         tau = on ? __uint_as_float(ld_cluster_u32(mapa_shared(smem_u32(&slip[par].tau), lane % 16))) : INFINITY;
         tau = -warp_max_nan(-tau);
       }
-    } else {
+    } else if (TOPK || wid * 32 < max(a.n_tok, 1)) {
       st = combine_lanes<ENT, false>(part[par][lane % NW], NW, a.c);
-      if (TOPK) tau = slip[par].tau;
     }
-    const bool bad = st.s != st.s;
     if (rank == 0 && t < max(a.n_tok, 1)) {
       const float ls = logf(st.s);
 #pragma unroll
@@ -582,120 +750,54 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
       if (ENT && t == 0 && a.entropy) a.entropy[r] = st.s == 0.f ? 0.f : ls - kLn2 * st.w / st.s;
     }
     if (TOPK) {
-      // f(z, id) for this thread's elements z >= least
-      auto each = [&](float least, auto f) {
-        for (int c = 0; c < chunks; ++c) {
-          if (!(cmax[c * NT + t] >= least)) continue;
-          for (int j = 0; j < kChunk; ++j) {
-            const int w = (c * kChunk + j) * NT + t;
-            if (w >= cur.n) break;
-            const uint4 q = buf[w];
-            if (!(Word<E>::template max<1>(&q) >= least)) continue;
-            const E *p = reinterpret_cast<const E *>(buf + w);
-            const int i0 = cur.id0(w);
-#pragma unroll
-            for (int k = 0; k < Word<E>::kN; ++k) {
-              const float z = Word<E>::one(p + k);
-              if (z >= least && i0 + k >= 0 && i0 + k < cur.V) f(z, i0 + k);
-            }
-          }
-        }
-      };
-      const uint32_t lead_count = C > 1 ? mapa_shared(smem_u32(&counts[0]), lead) : 0;
-      const uint32_t lead_cand = C > 1 ? mapa_shared(smem_u32(cand), lead) : 0;
-      auto collect = [&](float z, int id) {
-        if (C > 1) {
-          const unsigned i = atom_cluster_add_u32(lead_count, 1);
-          if (i < (unsigned)a.cap) st_cluster_u64(lead_cand + 8 * i, sort_key(z, id));
-        } else {
-          const int i = atomicAdd(&counts[0], 1);
-          if (i < a.cap) cand[i] = sort_key(z, id);
-        }
-      };
-      auto count = [&](int i) {  // counts[i] of the leader
-        return C > 1 ? (int)ld_cluster_u32(mapa_shared(smem_u32(&counts[i]), lead)) : counts[i];
-      };
-      if (!bad && tm >= tau) each(tau, collect);
-      sync();
-      int n = count(0);
-      if (n > a.cap) {
-        // too many (ties, few groups): bisect over whole keys to between k and cap of them
-        unsigned long long lo = sort_key(tau, INT_MAX), hi = ~0ull;
-        for (;;) {
-          const unsigned long long mid = lo + ((hi - lo) >> 1) + 1;
-          sync();
-          if (t == 0) counts[0] = counts[1] = 0;
-          sync();
-          int c = 0;
-          each(key_logit(mid), [&](float z, int id) { c += sort_key(z, id) >= mid; });
-          c = __reduce_add_sync(0xffffffffu, c);
-          if (lane == 0 && c) {
-            if (C > 1)
-              atom_cluster_add_u32(mapa_shared(smem_u32(&counts[1]), lead), (unsigned)c);
-            else
-              atomicAdd(&counts[1], c);
-          }
-          sync();
-          n = count(1);
-          if (n < a.top_k) {
-            hi = mid - 1;
-          } else {
-            lo = mid;
-            if (n <= a.cap) break;
-          }
-        }
-        each(key_logit(lo), [&](float z, int id) {
-          if (sort_key(z, id) >= lo) collect(z, id);
-        });
-        sync();
-      }
-      if (more)
-        for (int s = 0; s < kStages; ++s) nxt.load(s, cps, buf);
-      if (rank == lead) {
-        // order them: by counting when they are few, else a bitonic sort
-        int *ids = a.top_ids + (long long)r * a.top_k;
-        float *lps = a.top_logprob + (long long)r * a.top_k;
-        const float ls = logf(st.s);
-        if (bad) {
+      int *ids = a.top_ids + (long long)r * a.top_k;
+      float *lps = a.top_logprob + (long long)r * a.top_k;
+      if (st.s != st.s) {
+        if (rank == 0)
           for (int i = t; i < a.top_k; i += NT) ids[i] = -1, lps[i] = NAN;
-        } else if (n <= 192) {
-          for (int i = t; i < n; i += NT) {
-            const unsigned long long key = cand[i];
-            int above = 0;
-#pragma unroll 4
-            for (int j = 0; j + 1 < n; j += 2) {
-              const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(cand + j);
-              above += (v.x > key) + (v.y > key);
+      } else if (C == 1) {
+        put_greatest<NT>(cand, n, a.top_k, ids, lps, st.m, a.inv_t, st.s);
+      } else {
+        const uint32_t to_n = mapa_shared(smem_u32(&n_lead), 0), to = mapa_shared(smem_u32(gath), 0);
+        const uint32_t to_ge = mapa_shared(smem_u32(&n_ge), 0);
+        unsigned long long lo = sort_key(tau, INT_MAX), hi = ~0ull;
+        auto gather = [&] {
+          for (int i = t; i < n; i += NT)
+            if (cand[i] >= lo) {
+              const unsigned p = atom_cluster_add_u32(to_n, 1);
+              if (p < (unsigned)a.cap) st_cluster_u64(to + 8 * p, cand[i]);
             }
-            if (n & 1) above += cand[n - 1] > key;
-            if (above < a.top_k) {
-              ids[above] = key_id(key);
-              lps[above] = log_p(key_logit(key), st.m, a.inv_t, st.s, ls);
+        };
+        gather();
+        cluster_sync_all();
+        int m = (int)ld_cluster_u32(to_n);
+        if (m > a.cap) {  // ties over several slices: bisect
+          for (;;) {
+            const unsigned long long mid = lo + ((hi - lo) >> 1) + 1;
+            cluster_sync_all();
+            if (t == 0) n_ge = 0, n_lead = 0;
+            cluster_sync_all();
+            int g = 0;
+            for (int i = t; i < n; i += NT) g += cand[i] >= mid;
+            g = __reduce_add_sync(0xffffffffu, g);
+            if (lane == 0 && g) atom_cluster_add_u32(to_ge, (unsigned)g);
+            cluster_sync_all();
+            m = (int)ld_cluster_u32(to_ge);
+            if (m < a.top_k) {
+              hi = mid - 1;
+            } else {
+              lo = mid;
+              if (m <= a.cap) break;
             }
           }
-        } else {
-          int len = 256;
-          while (len < n) len *= 2;
-          for (int i = n + t; i < len; i += NT) cand[i] = 0;
-          for (int size = 2; size <= len; size *= 2)
-            for (int stride = size / 2; stride > 0; stride /= 2) {
-              __syncthreads();
-              for (int i = t; i < len / 2; i += NT) {
-                const int x = 2 * i - (i & (stride - 1)), y = x + stride;
-                const unsigned long long u = cand[x], v = cand[y];
-                if ((u < v) == ((x & size) == 0)) cand[x] = v, cand[y] = u;
-              }
-            }
-          __syncthreads();
-          for (int i = t; i < a.top_k; i += NT) {
-            const unsigned long long key = cand[i];
-            ids[i] = key_id(key);
-            lps[i] = log_p(key_logit(key), st.m, a.inv_t, st.s, ls);
-          }
+          gather();
+          cluster_sync_all();
         }
+        if (rank == 0) put_greatest<NT>(gath, m, a.top_k, ids, lps, st.m, a.inv_t, st.s);
       }
     }
-    cur = nxt;
+    if (r + step < a.in.rows) cur.next(a.in, r, step, rank);
+    r += step;
   }
   if (C > 1) cluster_sync_all();  // others may still read this CTA's slip
 }
@@ -800,6 +902,7 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_row_grad(const Row
   const int C = a.in.C;
   const unsigned rank = C > 1 ? cluster_ctarank() : 0;
   const int step = gridDim.x / C;
+  const float above = kAbove / fmaxf(a.c, LABEL1 ? kLog2E : 0.f);
   const int chunks = (a.in.wps + kChunk * NT - 1) / (kChunk * NT), cps = (chunks + kStages - 1) / kStages;
   const int nwl = min((ne + 31) / 32, NW);  // warps that hold entries
 
@@ -824,7 +927,8 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_row_grad(const Row
   for (int s = 0; s < kStages; ++s) load(cur, r, 0, s);
   for (; r < a.in.rows; r += step, par ^= 1) {
     const bool more = r + step < a.in.rows;
-    if (more) nxt.set(a.in, r + step, rank);
+    nxt = cur;
+    if (more) nxt.next(a.in, r, step, rank);
     const int *ids = ids2 + par * cap;
     const float *vals = vals2 + par * cap;
     const int V = a.in.V;
@@ -852,8 +956,8 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_row_grad(const Row
     auto stage = [&](int s) {
       for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
         uint4 q[kChunk];
-        cur.chunk(c, buf, q);
-        run.add(q, Word<E>::template max<kChunk>(q), a.c);
+        cur.chunk(c, buf + c * cur.kWide, q);
+        run.add(q, Word<E>::template max<kChunk>(q), a.c, above);
       }
     };
     copies_wait<3>(), stage(0);
@@ -1005,7 +1109,7 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_row_grad(const Row
     for (int s = 0; s < kStages; ++s) {
       for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
         uint4 q[kChunk];
-        cur.chunk(c, buf, q);
+        cur.chunk(c, buf + c * cur.kWide, q);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) {
           f2 v[kN / 2];
@@ -1180,26 +1284,46 @@ int check_grad(const char *who, const void *logits, int dtype, int rows, int voc
 // How rows are cut and spread.
 struct Plan {
   int wps, C, nt;
+  bool even;
 };
 
-// A row's slices hold at most 66 KB: three CTAs of an SM then have a row
-// each in flight or in work.  Longer rows go over a cluster of up to 8 CTAs,
-// then (few can be that long) slices grow to what one CTA can hold, then the
-// cluster to 16.  With fewer rows than SMs a row is spread further, down to
-// slices of 8 KB.
-Plan plan_rows(const void *logits, int dtype, int rows, int vocab, long long ld, size_t extra, int sms) {
+// What one row takes in 16-byte words, at most.
+int row_words(const void *logits, int dtype, int vocab, long long ld) {
   const int es = elem_size(dtype), kn = 16 / es;
-  const bool pitch = ld * es % 16 == 0;
-  const int pad = pitch ? (int)((reinterpret_cast<uintptr_t>(logits) & 15) / es) : kn - 1;
-  const int words = (pad + vocab + kn - 1) / kn;
+  const int pad = ld * es % 16 == 0 ? (int)((reinterpret_cast<uintptr_t>(logits) & 15) / es) : kn - 1;
+  return (pad + vocab + kn - 1) / kn;
+}
+
+// Streamed rows: a CTA a row, whatever its length.  When the rows leave SMs
+// short of CTAs a row is spread over a cluster of up to 8, down to slices of
+// 8 KB.
+Plan plan_stream(const void *logits, int dtype, int rows, int vocab, long long ld, int sms) {
+  const int words = row_words(logits, dtype, vocab, ld);
+  Plan p;
+  p.C = 1;
+  while (p.C < 8 && (long long)rows * p.C * 2 <= 2 * sms && words / (2 * p.C) >= 512) p.C *= 2;
+  p.wps = (words + p.C - 1) / p.C;
+  p.nt = p.wps <= 1024 ? 128 : 256;
+  p.even = ld * elem_size(dtype) % 16 == 0;
+  return p;
+}
+
+// Staged rows: a slice holds at most 66 KB, so that three CTAs of an SM have
+// a row each in flight or in work.  Longer rows go over a cluster of up to 8
+// CTAs, then (few can be that long) slices grow to what one CTA can hold,
+// then the cluster to 16.  With fewer rows than SMs a row is spread further,
+// down to slices of 8 KB.
+Plan plan_staged(const void *logits, int dtype, int rows, int vocab, long long ld, size_t extra, int sms) {
+  const int words = row_words(logits, dtype, vocab, ld);
   const size_t bytes = (size_t)words * 16, best = 66 * 1024, most = 224 * 1024 - extra;
   int C = (int)std::min<size_t>((bytes + best - 1) / best, 8);
   if ((bytes + C - 1) / C > most) C = 16;
-  while (C <= 4 && rows * C * 2 <= sms && bytes / (2 * C) >= 8192) C *= 2;
+  while (C <= 4 && (long long)rows * C * 2 <= sms && bytes / (2 * C) >= 8192) C *= 2;
   Plan p;
   p.C = C;
   p.wps = (words + C - 1) / C;
   p.nt = p.wps <= 1024 ? 128 : 256;
+  p.even = ld * elem_size(dtype) % 16 == 0;
   return p;
 }
 
@@ -1260,11 +1384,13 @@ int by_dtype(int dtype, F &&f) {
   return f(__half());
 }
 
-template <typename E, int NT>
+constexpr int kRing128 = 4, kRing256 = 3;  // chunks in flight a CTA
+
+template <typename E, int NT, int D>
 int score_nt(const char *who, const ScoreArgs &a, size_t smem, int dev, cudaStream_t st) {
-  if (a.top_k) return launch_rows(who, snai_score<E, NT, true, true>, a, NT, smem, dev, st);
-  if (a.entropy) return launch_rows(who, snai_score<E, NT, false, true>, a, NT, smem, dev, st);
-  return launch_rows(who, snai_score<E, NT, false, false>, a, NT, smem, dev, st);
+  if (a.top_k) return launch_rows(who, snai_score<E, NT, D, true, true>, a, NT, smem, dev, st);
+  if (a.entropy) return launch_rows(who, snai_score<E, NT, D, false, true>, a, NT, smem, dev, st);
+  return launch_rows(who, snai_score<E, NT, D, false, false>, a, NT, smem, dev, st);
 }
 
 // mode 0: scores' gradient, 1: distillation; extra: as the kernel's EXTRA
@@ -1280,9 +1406,10 @@ int grad_nt(const char *who, const RowGradArgs &a, int mode, bool extra, size_t 
 int launch_row_grad(const char *who, RowGradArgs &a, int dtype, int mode, bool extra, int dev, cudaStream_t st) {
   const int ne = a.n + (a.labels ? 1 : 0);
   const size_t lists = (size_t)((ne + 3) & ~3) * 6 * 4;
-  const Plan p = plan_rows(a.in.logits, dtype, a.in.rows, a.in.V, a.in.ld, lists, device_sm_count(dev));
+  const Plan p = plan_staged(a.in.logits, dtype, a.in.rows, a.in.V, a.in.ld, lists, device_sm_count(dev));
   a.in.wps = p.wps;
   a.in.C = p.C;
+  a.in.even = p.even;
   const size_t smem = (size_t)p.wps * 16 + lists;
   return by_dtype(dtype, [&](auto e) {
     using E = decltype(e);
@@ -1333,7 +1460,7 @@ int launch_score(const char *who, const ScoreLaunch &s, cudaStream_t stream) {
   if (dev < 0) return dev;
   DeviceGuard g(dev);
   ScoreArgs a{};
-  a.in = Rows{s.logits, s.ld, s.rows, s.V, 0, 0};
+  a.in = Rows{s.logits, s.ld, s.rows, s.V, 0, 0, false};
   a.tokens = s.tokens;
   a.n_tok = s.n_tok;
   a.c = (float)(1.4426950408889634 / s.temperature);
@@ -1343,18 +1470,19 @@ int launch_score(const char *who, const ScoreLaunch &s, cudaStream_t stream) {
   a.entropy = s.entropy;
   a.top_ids = s.top_ids;
   a.top_logprob = s.top_logprob;
-  // room for half again the alternatives: the threshold lets a quarter more groups through
-  if (s.top_k)
-    for (a.cap = 128; a.cap < s.top_k + s.top_k / 2 + 64;) a.cap *= 2;
-  const size_t lists = s.top_k ? (size_t)a.cap * 8 : 0;
-  const Plan p = plan_rows(s.logits, s.dtype, s.rows, s.V, s.ld, lists + 18 * 1024, device_sm_count(dev));
+  // thinned out at twice the alternatives; room for as many again in one chunk
+  a.soft = std::max(96, 2 * s.top_k + 32);
+  for (a.cap = 256; a.cap < a.soft + a.soft / 2;) a.cap *= 2;
+  const Plan p = plan_stream(s.logits, s.dtype, s.rows, s.V, s.ld, device_sm_count(dev));
   a.in.wps = p.wps;
   a.in.C = p.C;
-  const size_t maxima = ((size_t)((p.wps + kChunk * p.nt - 1) / (kChunk * p.nt)) + 1) * p.nt * 4;
-  const size_t smem = (size_t)p.wps * 16 + (s.top_k ? lists + maxima : 0);
+  a.in.even = p.even;
+  const size_t lists = s.top_k ? (size_t)a.cap * 8 * (p.C > 1 ? 2 : 1) + (size_t)kChunk * p.nt * 4 : 0;
+  const size_t smem = (size_t)(p.nt == 128 ? kRing128 : kRing256) * kChunk * p.nt * 16 + lists;
   return by_dtype(s.dtype, [&](auto e) {
     using E = decltype(e);
-    return p.nt == 128 ? score_nt<E, 128>(who, a, smem, dev, stream) : score_nt<E, 256>(who, a, smem, dev, stream);
+    return p.nt == 128 ? score_nt<E, 128, kRing128>(who, a, smem, dev, stream)
+                       : score_nt<E, 256, kRing256>(who, a, smem, dev, stream);
   });
 }
 
@@ -1400,7 +1528,7 @@ int launch_distill(const char *who, const DistillLaunch &s, cudaStream_t stream)
   if (dev < 0) return dev;
   DeviceGuard g(dev);
   RowGradArgs a{};
-  a.in = Rows{s.logits, s.ld, s.rows, s.V, 0, 0};
+  a.in = Rows{s.logits, s.ld, s.rows, s.V, 0, 0, false};
   a.ids = s.teacher_ids;
   a.vals = s.teacher_logits;
   a.n = s.top_k;
@@ -1474,7 +1602,7 @@ extern "C" int cortex_score_grad(const void *logits, int dtype, int rows, int vo
   if (dev < 0) return dev;
   DeviceGuard g(dev);
   RowGradArgs a{};
-  a.in = Rows{logits, ld, rows, vocab, 0, 0};
+  a.in = Rows{logits, ld, rows, vocab, 0, 0, false};
   a.ids = tokens;
   a.vals = g_logprob;
   a.n = n_tok;
