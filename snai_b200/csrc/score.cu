@@ -216,6 +216,26 @@ struct Rows {
   bool even;  // all rows start at the same place of a 16-byte word
 };
 
+// The word at p whose element 0 is id0 of a row of V, -inf beyond the row's
+// ends; and such a word's elements to the row at out.  By value, and not
+// members: an object whose address a call takes lives in local memory.
+template <typename E>
+__device__ __noinline__ uint4 ragged(const char *p, int id0, int V) {
+  __align__(16) E v[Word<E>::kN];
+#pragma unroll
+  for (int k = 0; k < Word<E>::kN; ++k)
+    Word<E>::put(v + k,
+                 id0 + k >= 0 && id0 + k < V ? Word<E>::one(reinterpret_cast<const E *>(p) + k) : -INFINITY);
+  return *reinterpret_cast<const uint4 *>(v);
+}
+template <typename E>
+__device__ __noinline__ void put_ragged(uint4 q, E *out, int id0, int V) {
+  const E *v = reinterpret_cast<const E *>(&q);
+#pragma unroll
+  for (int k = 0; k < Word<E>::kN; ++k)
+    if (id0 + k >= 0 && id0 + k < V) out[id0 + k] = v[k];
+}
+
 // One CTA's slice of one row: words [first, first + n) of the row's 16-byte
 // grid, which starts `pad` elements before the row when the row does not
 // start on a word.  Thread t owns words t, t + NT, ... of the slice.  All
@@ -272,7 +292,7 @@ struct Slice {
         if (w >= lo && w < hi)
           copy16(dst + j * NT * 16, p + j * NT * 16);
         else if (w < n)
-          ragged(w, to + (w - w0));
+          to[w - w0] = ragged<E>(p + j * NT * 16, id0(w), V);
       }
     }
   }
@@ -285,17 +305,15 @@ struct Slice {
   __device__ static __forceinline__ void copy16(uint32_t dst, const char *p) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(p) : "memory");
   }
-  __device__ __noinline__ void ragged(int w, uint4 *to) const {
-    E *p = reinterpret_cast<E *>(to);
-    const int i0 = id0(w);
-    for (int k = 0; k < kN; ++k) Word<E>::put(p + k, i0 + k >= 0 && i0 + k < V ? Word<E>::one(at(i0 + k)) : -INFINITY);
+  // word w from global memory, masked beyond the row's ends
+  __device__ __forceinline__ uint4 fetch(int w) const {
+    const char *p = src + (long long)w * 16;
+    if (w >= lo && w < hi) return *reinterpret_cast<const uint4 *>(p);
+    return ragged<E>(p, id0(w), V);
   }
-  // out: the output row's element 0
-  __device__ __noinline__ void store_ragged(int w, uint4 q, E *out) const {
-    const E *p = reinterpret_cast<const E *>(&q);
-    const int i0 = id0(w);
-    for (int k = 0; k < kN; ++k)
-      if (i0 + k >= 0 && i0 + k < V) out[i0 + k] = p[k];
+  // stores word w of a row whose element 0 is at out
+  __device__ __forceinline__ void store_ragged(int w, const uint4 &q, E *out) const {
+    put_ragged(q, out, id0(w), V);
   }
   // this thread's four words of chunk c, staged at `at` (all masked past the slice's end)
   __device__ __forceinline__ void chunk(int c, const uint4 *at, uint4 *q) const {
@@ -421,7 +439,7 @@ struct ScoreArgs {
   const int *tokens;
   int n_tok;
   float c, inv_t;  // log2(e) / T, 1 / T
-  int top_k, cap, soft;  // candidates: what the buffer holds (a power of two), and where it is thinned out
+  int top_k, cap, soft, grow;  // candidates: what the buffer holds (a power of two), where it is thinned out, and when
   float *logprob, *entropy;
   int *top_ids;
   float *top_logprob;
@@ -431,31 +449,53 @@ __device__ __forceinline__ float log_p(float z, float m, float inv_t, float s, f
   return s == 0.f || z == -INFINITY ? -INFINITY + (s - s) : (z - m) * inv_t - ls;
 }
 
-// A value that at least k of n values reach and few more do, by one warp:
-// their k-th largest, or a little less.  -inf when n < k.  at(i) is the i-th
-// value; N values a lane are held in registers (N = 0: fetched each time).
-template <int N, class At>
-__device__ __forceinline__ float about_kth(At at, int n, int k) {
+// The next float up, past both zeros.
+__device__ __forceinline__ float next_up(float v) {
+  const int b = __float_as_int(v + 0.0f);
+  return __int_as_float(b >= 0 ? b + 1 : b - 1);
+}
+
+// Loads that stay where they are written: ahead of the work that hides them.
+__device__ __forceinline__ int load_now(const int *p) {
+  int v;
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float load_now(const float *p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float load_now(const __nv_bfloat16 *p) {
+  unsigned short v;
+  asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
+  return __uint_as_float((unsigned)v << 16);
+}
+__device__ __forceinline__ float load_now(const __half *p) {
+  unsigned short v;
+  asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
+  return __half2float(__ushort_as_half(v));
+}
+
+// Floats as integers of the same order, and back.
+__device__ __forceinline__ int ordered(float v) {
+  const int b = __float_as_int(v);
+  return b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float unordered(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
+
+// A value that at least k of n values reach and few more do (their k-th
+// largest, or a little less), by one warp; -inf when n < k.  The values are
+// ordered integers, `pitch` of them apart (1: an array of them, 2: the upper
+// halves of sort keys, whose order has its sign bit flipped).
+__device__ __noinline__ float about_kth(const int *v, int pitch, int n, int k) {
   if (n < k) return -INFINITY;
-  const int lane = threadIdx.x & 31;
-  auto ordered = [](float v) {
-    const int b = __float_as_int(v);
-    return b ^ ((b >> 31) & 0x7fffffff);
-  };
-  int v[N ? N : 1];
+  const int lane = threadIdx.x & 31, flip = pitch == 2 ? (int)0x80000000 : 0;
   int lo = 0x7fffffff, hi = (int)0x80000000;
-  if (N) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[i] = ordered(i * 32 + lane < n ? at(i * 32 + lane) : -INFINITY);
-      if (i * 32 + lane < n) lo = min(lo, v[i]);
-      hi = max(hi, v[i]);
-    }
-  } else {
-    for (int i = lane; i < n; i += 32) {
-      const int x = ordered(at(i));
-      lo = min(lo, x), hi = max(hi, x);
-    }
+#pragma unroll 4
+  for (int i = lane; i < n; i += 32) {
+    const int x = v[i * pitch] ^ flip;
+    lo = min(lo, x), hi = max(hi, x);
   }
   lo = __reduce_min_sync(0xffffffffu, lo);  // k values reach lo
   hi = __reduce_max_sync(0xffffffffu, hi);
@@ -463,12 +503,8 @@ __device__ __forceinline__ float about_kth(At at, int n, int k) {
   while (lo < hi) {
     const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) >> 1);
     int c = 0;
-    if (N) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) c += v[i] >= mid;
-    } else {
-      for (int i = lane; i < n; i += 32) c += ordered(at(i)) >= mid;
-    }
+#pragma unroll 8
+    for (int i = lane; i < n; i += 32) c += (v[i * pitch] ^ flip) >= mid;
     c = __reduce_add_sync(0xffffffffu, c);
     if (c >= k) {
       lo = mid;
@@ -477,49 +513,149 @@ __device__ __forceinline__ float about_kth(At at, int n, int k) {
       hi = mid - 1;
     }
   }
-  return __int_as_float(lo ^ ((lo >> 31) & 0x7fffffff));
+  return unordered(max(lo, (int)0x807fffff));  // -inf: below it lie no logits, only the empty keys of a buffer
+}
+__device__ __forceinline__ const int *upper_halves(const unsigned long long *keys) {
+  return reinterpret_cast<const int *>(keys) + 1;
+}
+
+// Bitonic sort of n keys, descending; room for the next power of two.  The
+// whole block calls it.
+template <int NT>
+__device__ __noinline__ void sort_keys(unsigned long long *key, int n) {
+  int len = 512;
+  while (len < n) len *= 2;
+  for (int i = n + (int)threadIdx.x; i < len; i += NT) key[i] = 0;
+  for (int size = 2; size <= len; size *= 2)
+    for (int stride = size / 2; stride > 0; stride /= 2) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < len / 2; i += NT) {
+        const int x = 2 * i - (i & (stride - 1)), y = x + stride;
+        const unsigned long long u = key[x], v = key[y];
+        if ((u < v) == ((x & size) == 0)) key[x] = v, key[y] = u;
+      }
+    }
+  __syncthreads();
 }
 
 // Writes the k greatest of n keys (k <= n; ids and log p, in order): by
-// counting the greater ones when they are few, else by a bitonic sort (cand
-// holds a power of two of at least n keys).  The whole block calls it.
+// counting the greater ones when they are few, else by a sort.  The whole
+// block calls it.
 template <int NT>
 __device__ __forceinline__ void put_greatest(unsigned long long *cand, int n, int k, int *ids, float *lps, float m,
                                              float inv_t, float s) {
   const int t = threadIdx.x;
+  const bool sorted = n > 384;
+  if (sorted) sort_keys<NT>(cand, n);
   const float ls = logf(s);
-  auto put = [&](int i, unsigned long long key) {
-    ids[i] = key_id(key);
-    lps[i] = log_p(key_logit(key), m, inv_t, s, ls);
-  };
-  if (n <= 256) {
-    for (int i = t; i < n; i += NT) {
-      const unsigned long long key = cand[i];
-      int above = 0;
+  for (int i = t; i < (sorted ? k : n); i += NT) {
+    const unsigned long long key = cand[i];
+    int at = i;
+    if (!sorted) {
+      at = n & 1 ? cand[n - 1] > key : 0;
 #pragma unroll 4
       for (int j = 0; j + 1 < n; j += 2) {
         const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(cand + j);
-        above += (v.x > key) + (v.y > key);
+        at += (v.x > key) + (v.y > key);
       }
-      if (n & 1) above += cand[n - 1] > key;
-      if (above < k) put(above, key);
     }
-    return;
+    if (at < k) {
+      ids[at] = key_id(key);
+      lps[at] = log_p(key_logit(key), m, inv_t, s, ls);
+    }
   }
-  int len = 512;
-  while (len < n) len *= 2;
-  for (int i = n + t; i < len; i += NT) cand[i] = 0;
-  for (int size = 2; size <= len; size *= 2)
-    for (int stride = size / 2; stride > 0; stride /= 2) {
-      __syncthreads();
-      for (int i = t; i < len / 2; i += NT) {
-        const int x = 2 * i - (i & (stride - 1)), y = x + stride;
-        const unsigned long long u = cand[x], v = cand[y];
-        if ((u < v) == ((x & size) == 0)) cand[x] = v, cand[y] = u;
-      }
-    }
+}
+
+// What the block's threads share of a row's candidates.
+struct Pool {
+  unsigned long long *key;  // cap of them
+  int *n;                   // collected (may pass cap)
+  int *ge;
+  float *tau;
+  int cap;
+};
+
+// Thins out a pool of n <= cap candidates: about the k greatest stay; returns
+// the value they reach.  The whole block calls it, after a barrier.
+template <int NT>
+__device__ __noinline__ float thin_out(const Pool p, int n, int k) {
+  const int t = threadIdx.x;
+  if (t < 32) {
+    const float b = about_kth(upper_halves(p.key), 2, n, k);
+    if (t == 0) *p.tau = b, *p.n = 0;
+  }
   __syncthreads();
-  for (int i = t; i < k; i += NT) put(i, cand[i]);
+  const float tau = *p.tau;
+  unsigned long long own[kMaxCap / NT];
+  int m = 0;
+#pragma unroll
+  for (int i = 0; i < kMaxCap / NT; ++i) {
+    own[i] = i * NT + t < n ? p.key[i * NT + t] : 0;
+    if (key_logit(own[i]) >= tau)  // an empty key is no number
+      ++m;
+    else
+      own[i] = 0;
+  }
+  __syncthreads();
+  int at = m ? atomicAdd(p.n, m) : 0;
+#pragma unroll
+  for (int i = 0; i < kMaxCap / NT; ++i)
+    if (own[i]) p.key[at++] = own[i];
+  __syncthreads();
+  return tau;
+}
+
+// f(z, id) for this thread's logits >= least of `words` words a thread, the
+// first of them w0 + thread; word(w) gives the staged or loaded word w.
+template <typename E, int NT, class Get, class F>
+__device__ __forceinline__ void each_logit(const Slice<E, NT> &s, int w0, int words, float least, Get word, F f) {
+  for (int j = 0; j < words; ++j) {
+    const int w = w0 + j * NT + (int)threadIdx.x;
+    if (w >= s.n) break;
+    const uint4 q = word(w);
+    if (!(Word<E>::template max<1>(&q) >= least)) continue;
+    const E *p = reinterpret_cast<const E *>(&q);
+    for (int k = 0; k < Word<E>::kN; ++k) {
+      const float z = Word<E>::one(p + k);
+      const int id = s.id0(w) + k;
+      if (z >= least && id >= 0 && id < s.V) f(z, id);
+    }
+  }
+}
+
+// More candidates than the pool holds (rows of few values, or ascending
+// ones): the pool becomes between k and `few` keys that hold the k greatest
+// of the slice's words [w0, w0 + words * NT), by bisection over whole keys
+// from `tau` on; each reading takes the words again.  Returns the value they
+// all reach.  The whole block calls it, after a barrier.
+template <typename E, int NT, class Get>
+__device__ __noinline__ float cut_out(const Pool p, const Slice<E, NT> s, int w0, int words, float tau, int k, int few,
+                                      Get word) {
+  const int t = threadIdx.x;
+  unsigned long long lo = sort_key(tau, INT_MAX), hi = ~0ull;
+  for (;;) {
+    const unsigned long long mid = lo + ((hi - lo) >> 1) + 1;
+    __syncthreads();
+    if (t == 0) *p.ge = *p.n = 0;
+    __syncthreads();
+    int g = 0;
+    each_logit(s, w0, words, key_logit(mid), word, [&](float z, int id) { g += sort_key(z, id) >= mid; });
+    g = __reduce_add_sync(0xffffffffu, g);
+    if ((t & 31) == 0 && g) atomicAdd(p.ge, g);
+    __syncthreads();
+    g = *p.ge;
+    if (g < k) {
+      hi = mid - 1;
+    } else {
+      lo = mid;
+      if (g <= few) break;
+    }
+  }
+  each_logit(s, w0, words, key_logit(lo), word, [&](float z, int id) {
+    if (sort_key(z, id) >= lo) p.key[atomicAdd(p.n, 1)] = sort_key(z, id);
+  });
+  __syncthreads();
+  return key_logit(lo);
 }
 
 // Rows stream through a ring of D chunks of shared memory: a thread waits for
@@ -527,14 +663,17 @@ __device__ __forceinline__ void put_greatest(unsigned long long *cand, int n, in
 // row or the next.
 //
 // Alternatives are found on the way, in one reading.  From the first chunk's
-// maxima (of each thread's words, or of each word when k is large) comes a
+// maxima (of each thread's four, two or single words, as k grows) comes a
 // value tau that at least k logits reach; what reaches it is a candidate.  In
 // later chunks only logits above tau can be alternatives, since equal ones
-// have greater ids than k others.  When the candidates pass a soft limit tau
-// is raised to about their k-th greatest and the rest dropped; a chunk that
-// brings more than the buffer holds (rows of equal or ascending logits) is
-// cut exactly, by bisection over (logit, id) keys.  What remains is ordered
-// at the row's end.
+// have greater ids than k others.  After the first chunk, and each time the
+// row has grown `grow` times since, the block meets and, when the candidates
+// are half again as many as k, raises tau to about their k-th greatest and
+// drops the rest; in between its warps run on their own.  More candidates than the
+// buffer holds are cut out exactly: those of the first chunk from its staged
+// words (rows of few values, or masked but for fewer than k), those of a row
+// whose logits keep rising by reading it again.  What remains is ordered at
+// the row's end.
 //
 // A row over a cluster (few rows) has each slice find its own candidates;
 // those that reach the least of the slices' about ceil(k / C)-th greatest are
@@ -551,14 +690,14 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
   // candidates, then (rank 0 of a cluster) those of all slices, then the first chunk's maxima
   unsigned long long *cand = reinterpret_cast<unsigned long long *>(smem + D * kWide * 16);
   unsigned long long *gath = cand + a.cap;
-  float *maxima = reinterpret_cast<float *>(gath + (a.in.C > 1 ? a.cap : 0));
+  int *maxima = reinterpret_cast<int *>(gath + (a.in.C > 1 ? a.cap : 0));
+  const Pool pool = {cand, &n_cand, &n_ge, &tau_s, a.cap};
   const int t = threadIdx.x, lane = t & 31, wid = t >> 5;
   const int C = a.in.C;
   const unsigned rank = C > 1 ? cluster_ctarank() : 0;
   const int step = gridDim.x / C;
   const int chunks = (a.in.wps + kWide - 1) / kWide;
   const float above = kAbove / a.c;
-  const bool by_word = 4 * a.top_k > NT;
 
   Slice<E, NT> cur, ahead;  // the row in work, the row being sent for
   int r = blockIdx.x / C, ra = r, ca = 0, slot = 0;
@@ -575,25 +714,32 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
     }
     ahead.commit();
   };
+  int tok[kMaxList / NT];
+  auto next_tokens = [&](int row) {
+#pragma unroll
+    for (int i = 0; i < kMaxList / NT; ++i) {
+      const int j = i * NT + t;
+      tok[i] = j < a.n_tok ? load_now(a.tokens + (long long)row * a.n_tok + j) : -1;
+    }
+  };
+  if (rank == 0 && wid * 32 < a.n_tok) next_tokens(r);
   for (int i = 0; i < D; ++i) send(ring + i * kWide);
   int par = 0;
   for (; r < a.in.rows; par ^= 1) {
-    // the tokens' logits, read beside the row's copies
+    // the tokens' logits, read beside the row's copies; the next row's tokens
     float zt[kMaxList / NT];
     bool in[kMaxList / NT];
-    if (rank == 0)
+    if (rank == 0 && wid * 32 < a.n_tok) {
 #pragma unroll
       for (int i = 0; i < kMaxList / NT; ++i) {
-        const int j = i * NT + t;
-        zt[i] = 0.f, in[i] = false;
-        if (j < a.n_tok) {
-          const int id = a.tokens[(long long)r * a.n_tok + j];
-          in[i] = id >= 0 && id < a.in.V;
-          if (in[i]) zt[i] = Word<E>::one(cur.at(id));
-        }
+        in[i] = tok[i] >= 0 && tok[i] < a.in.V;
+        zt[i] = in[i] ? load_now(cur.at(tok[i])) : 0.f;
       }
+      if (r + step < a.in.rows) next_tokens(r + step);
+    }
     Running<E, ENT, false> run;
-    float tau = -INFINITY;
+    float tau = -INFINITY, least = -INFINITY;  // of a chunk's logits, those from `least` on are candidates
+    int meet = 0;                              // the chunk after which the block meets next
     for (int c = 0; c < chunks; ++c) {
       uint4 *at = ring + slot * kWide;
       slot = slot + 1 == D ? 0 : slot + 1;
@@ -603,117 +749,59 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
       const float cm = Word<E>::template max<kChunk>(q);
       run.add(q, cm, a.c, above);
       if (TOPK) {
-        const int w0 = c * kWide + t;
-        // f(z, id) for this thread's logits of the chunk that reach `least`
-        auto each = [&](float least, auto f) {
-          for (int j = 0; j < kChunk; ++j) {
-            if (w0 + j * NT >= cur.n) break;
-            const uint4 w = at[j * NT + t];
-            if (!(Word<E>::template max<1>(&w) >= least)) continue;
-            const E *p = reinterpret_cast<const E *>(at + j * NT + t);
-            const int i0 = cur.id0(w0 + j * NT);
-            for (int k = 0; k < kN; ++k) {
-              const float z = Word<E>::one(p + k);
-              if (z >= least && i0 + k >= 0 && i0 + k < cur.V) f(z, i0 + k);
-            }
-          }
-        };
-        int last = -1;  // this thread's last place in the buffer
-        auto push = [&](unsigned long long key) {
-          last = atomicAdd(&n_cand, 1);
-          if (last < a.cap) cand[last] = key;
-        };
-        bool full;
         if (c == 0) {
-          if (by_word) {
+          // groups of four words (a thread's), two, or one
+          const int per = 4 * a.top_k <= NT ? 1 : 4 * a.top_k <= 2 * NT ? 2 : 4;
+          maxima[t] = ordered(per == 1 ? cm : Word<E>::template max<1>(q));
+          if (per == 2) {
+            maxima[t] = ordered(Word<E>::template max<2>(q));
+            maxima[NT + t] = ordered(Word<E>::template max<2>(q + 2));
+          } else if (per == 4) {
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) maxima[j * NT + t] = Word<E>::template max<1>(q + j);
-          } else {
-            maxima[t] = cm;
+            for (int j = 1; j < kChunk; ++j) maxima[j * NT + t] = ordered(Word<E>::template max<1>(q + j));
           }
           __syncthreads();
           if (wid == 0) {
-            auto val = [&](int i) { return maxima[i]; };
-            const float b = by_word ? about_kth<0>(val, kChunk * NT, a.top_k) : about_kth<NT / 32>(val, NT, a.top_k);
+            const float b = about_kth(maxima, 1, per * NT, a.top_k);
             if (lane == 0) tau_s = b, n_cand = 0;
           }
           __syncthreads();
-          tau = tau_s;
-          if (cm >= tau) each(tau, [&](float z, int id) { push(sort_key(z, id)); });
-        } else if (cm > tau) {
-          each(tau, [&](float z, int id) {
-            if (z > tau) push(sort_key(z, id));
-          });
+          tau = least = tau_s;
         }
-        full = __syncthreads_or(last >= a.soft);
-        if (full) {
-          const int n = n_cand;
-          __syncthreads();
-          if (n <= a.cap) {
-            // drop what cannot be among the k greatest
-            if (wid == 0) {
-              const float b = about_kth<0>([&](int i) { return key_logit(cand[i]); }, n, a.top_k);
-              if (lane == 0) tau_s = b, n_cand = 0;
+        if (cm >= least) {
+          // this thread's hits as bits, room for them, then their keys
+          unsigned hits = 0;
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) {
+            f2 v[kN / 2];
+            Word<E>::unpack(q[j], v);
+#pragma unroll
+            for (int k = 0; k < kN / 2; ++k) {
+              float x, y;
+              unpack2(v[k], x, y);
+              hits |= (x >= least ? 1u << (j * kN + 2 * k) : 0u) | (y >= least ? 2u << (j * kN + 2 * k) : 0u);
             }
-            __syncthreads();
-            tau = tau_s;
-            unsigned long long own[kMaxCap / NT];
-            int m = 0;
-#pragma unroll
-            for (int i = 0; i < kMaxCap / NT; ++i) {
-              own[i] = i * NT + t < n ? cand[i * NT + t] : 0;
-              if (i * NT + t < n && key_logit(own[i]) >= tau)
-                ++m;
-              else
-                own[i] = 0;
-            }
-            __syncthreads();
-            int p = m ? atomicAdd(&n_cand, m) : 0;
-#pragma unroll
-            for (int i = 0; i < kMaxCap / NT; ++i)
-              if (own[i]) cand[p++] = own[i];
-            __syncthreads();
-          } else {
-            // more than the buffer holds: the candidates of earlier chunks
-            // and all of this one, cut to between k and cap
-            const int floor_id = c == 0 ? 0 : cur.id0(c * kWide);
-            unsigned long long lo = sort_key(tau, INT_MAX), hi = ~0ull;
-            auto old = [&](int i) { return key_id(cand[i]) < floor_id ? cand[i] : 0ull; };
-            for (;;) {
-              const unsigned long long mid = lo + ((hi - lo) >> 1) + 1;
-              __syncthreads();
-              if (t == 0) n_ge = 0;
-              __syncthreads();
-              int g = 0;
-              for (int i = t; i < a.cap; i += NT) g += old(i) >= mid;
-              each(key_logit(mid), [&](float z, int id) { g += sort_key(z, id) >= mid; });
-              g = __reduce_add_sync(0xffffffffu, g);
-              if (lane == 0 && g) atomicAdd(&n_ge, g);
-              __syncthreads();
-              g = n_ge;
-              if (g < a.top_k) {
-                hi = mid - 1;
-              } else {
-                lo = mid;
-                if (g <= a.soft) break;
-              }
-            }
-            unsigned long long own[kMaxCap / NT];
-#pragma unroll
-            for (int i = 0; i < kMaxCap / NT; ++i) own[i] = i * NT + t < a.cap ? old(i * NT + t) : 0;
-            __syncthreads();
-            if (t == 0) n_cand = 0;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kMaxCap / NT; ++i)
-              if (own[i] >= lo) push(own[i]);
-            each(key_logit(lo), [&](float z, int id) {
-              if (sort_key(z, id) >= lo) push(sort_key(z, id));
-            });
-            tau = key_logit(lo);
-            __syncthreads();
+          }
+          for (int p = atomicAdd(&n_cand, __popc(hits)); hits; hits &= hits - 1, ++p) {
+            const int b = __ffs(hits) - 1, j = b / kN, k = b % kN, id = cur.id0(c * kWide + j * NT + t) + k;
+            const float z = Word<E>::one(reinterpret_cast<const E *>(at + j * NT + t) + k);
+            // the masked filling behind the row's ends is no logit: an empty key
+            if (p < a.cap) cand[p] = id >= 0 && id < cur.V ? sort_key(z, id) : 0;
           }
         }
+        if (c == meet || c == chunks - 1) {
+          __syncthreads();
+          const int n = n_cand;
+          __syncthreads();
+          if (n > a.cap)
+            tau = c == 0 ? cut_out<E, NT>(pool, cur, 0, kChunk, tau, a.top_k, a.soft, [at](int w) { return at[w]; })
+                         : cut_out<E, NT>(pool, cur, 0, (c + 1) * kChunk, tau, a.top_k, a.soft,
+                                          [cur](int w) { return cur.fetch(w); });
+          else if (n > a.soft && c < chunks - 1)
+            tau = thin_out<NT>(pool, n, a.top_k);
+          meet = a.grow * (meet + 1) - 1;
+        }
+        least = next_up(tau);
       }
       send(at);
     }
@@ -726,7 +814,7 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
         st = combine_lanes<ENT, false>(part[par][lane % NW], NW, a.c);
         if (TOPK)
           tau = st.s != st.s ? INFINITY
-                             : about_kth<0>([&](int i) { return key_logit(cand[i]); }, n, (a.top_k + C - 1) / C);
+                             : about_kth(upper_halves(cand), 2, n, (a.top_k + C - 1) / C);
         if (lane == 0) slip[par].st = st, slip[par].tau = tau, n_lead = 0;
       }
       cluster_sync_all();
@@ -1470,9 +1558,12 @@ int launch_score(const char *who, const ScoreLaunch &s, cudaStream_t stream) {
   a.entropy = s.entropy;
   a.top_ids = s.top_ids;
   a.top_logprob = s.top_logprob;
-  // thinned out at twice the alternatives; room for as many again in one chunk
-  a.soft = std::max(96, 2 * s.top_k + 32);
-  for (a.cap = 256; a.cap < a.soft + a.soft / 2;) a.cap *= 2;
+  // A value that 1.25 k logits of a part of the row reach is reached by about
+  // 3.75 k more of four times as much: with room for 6 k the block meets each
+  // time the row has grown fourfold, else each time it has doubled.
+  a.soft = s.top_k + s.top_k / 2 + 16;
+  for (a.cap = 256; a.cap < kMaxCap && a.cap < 6 * s.top_k;) a.cap *= 2;
+  a.grow = a.cap >= 6 * s.top_k ? 4 : 2;
   const Plan p = plan_stream(s.logits, s.dtype, s.rows, s.V, s.ld, device_sm_count(dev));
   a.in.wps = p.wps;
   a.in.C = p.C;
