@@ -95,6 +95,13 @@ __device__ __forceinline__ float sum2(f2 v) {
   return a + b;
 }
 
+// Eight bits, in order, from four pairs of 16-bit masks.
+__device__ __forceinline__ unsigned reach8(unsigned a, unsigned b, unsigned c, unsigned d) {
+  // pair i's low half gives bit 2 i, its high half bit 16 + 2 i + 1
+  const unsigned v = (a & 0x00020001u) | (b & 0x00080004u) | (c & 0x00200010u) | (d & 0x00800040u);
+  return (v | v >> 16) & 0xffu;
+}
+
 // A 16-byte word of logits: kN elements; kMasked is -inf in each of its 32-bit parts.
 template <typename E> struct Word;
 template <> struct Word<float> {
@@ -119,6 +126,13 @@ template <> struct Word<float> {
       m = max_nan(m, max_nan(__uint_as_float(q[j].z), __uint_as_float(q[j].w)));
     }
     return m;
+  }
+  // one bit for each element that reaches limit(least)
+  __device__ static __forceinline__ unsigned limit(float least) { return __float_as_uint(least); }
+  __device__ static __forceinline__ unsigned reach(const uint4 &w, unsigned lim) {
+    const float l = __uint_as_float(lim);
+    return (__uint_as_float(w.x) >= l ? 1u : 0u) | (__uint_as_float(w.y) >= l ? 2u : 0u) |
+           (__uint_as_float(w.z) >= l ? 4u : 0u) | (__uint_as_float(w.w) >= l ? 8u : 0u);
   }
   __device__ static __forceinline__ float one(const float *p) { return *p; }
   __device__ static __forceinline__ void put(float *p, float v) { *p = v; }
@@ -152,6 +166,16 @@ template <> struct Word<__nv_bfloat16> {
 #pragma unroll
     for (int j = 0; j < N; ++j) m = max2(m, max2(max2(q[j].x, q[j].y), max2(q[j].z, q[j].w)));
     return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  }
+  __device__ static __forceinline__ unsigned limit(float least) {
+    const __nv_bfloat162 v = __bfloat162bfloat162(__float2bfloat16_ru(least));
+    return *reinterpret_cast<const unsigned *>(&v);
+  }
+  __device__ static __forceinline__ unsigned ge2(unsigned a, unsigned lim) {
+    return __hge2_mask(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&lim));
+  }
+  __device__ static __forceinline__ unsigned reach(const uint4 &w, unsigned lim) {
+    return reach8(ge2(w.x, lim), ge2(w.y, lim), ge2(w.z, lim), ge2(w.w, lim));
   }
   __device__ static __forceinline__ float one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
   __device__ static __forceinline__ void put(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
@@ -188,6 +212,16 @@ template <> struct Word<__half> {
     float a, b;
     unpack2(two(m), a, b);
     return max_nan(a, b);
+  }
+  __device__ static __forceinline__ unsigned limit(float least) {
+    const __half2 v = __half2half2(__float2half_ru(least));
+    return *reinterpret_cast<const unsigned *>(&v);
+  }
+  __device__ static __forceinline__ unsigned ge2(unsigned a, unsigned lim) {
+    return __hge2_mask(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&lim));
+  }
+  __device__ static __forceinline__ unsigned reach(const uint4 &w, unsigned lim) {
+    return reach8(ge2(w.x, lim), ge2(w.y, lim), ge2(w.z, lim), ge2(w.w, lim));
   }
   __device__ static __forceinline__ float one(const __half *p) { return __half2float(*p); }
   __device__ static __forceinline__ void put(__half *p, float v) { *p = __float2half_rn(v); }
@@ -484,6 +518,44 @@ __device__ __forceinline__ int ordered(float v) {
 }
 __device__ __forceinline__ float unordered(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
 
+// A value that at least k <= 32 N of the warp's 32 N values reach and few
+// more do.  Few: the greatest are taken off one after the other; else
+// bisection, ended a little early.
+template <int N>
+__device__ __forceinline__ float warp_kth(const float *v, int k) {
+  int x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = ordered(v[i]);
+  if (N == 1 && k <= 8) {
+    int top, c = 0;
+    do {
+      top = __reduce_max_sync(0xffffffffu, x[0]);
+      c += __popc(__ballot_sync(0xffffffffu, x[0] == top));
+      if (x[0] == top) x[0] = (int)0x80000000;
+    } while (c < k);
+    return unordered(max(top, (int)0x807fffff));
+  }
+  int lo = x[0], hi = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) lo = min(lo, x[i]), hi = max(hi, x[i]);
+  lo = __reduce_min_sync(0xffffffffu, lo);  // all values reach lo
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  while (lo < hi) {
+    const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) >> 1);
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) c += x[i] >= mid;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= k) {
+      lo = mid;
+      if (c <= k + (k >> 3)) break;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  return unordered(max(lo, (int)0x807fffff));
+}
+
 // A value that at least k of n values reach and few more do (their k-th
 // largest, or a little less), by one warp; -inf when n < k.  The values are
 // ordered integers, `pitch` of them apart (1: an array of them, 2: the upper
@@ -663,13 +735,12 @@ __device__ __noinline__ float cut_out(const Pool p, const Slice<E, NT> s, int w0
 // row or the next.
 //
 // Alternatives are found on the way, in one reading.  From the first chunk's
-// maxima (of each thread's four, two or single words, as k grows) comes a
-// value tau that at least k logits reach; what reaches it is a candidate.  In
-// later chunks only logits above tau can be alternatives, since equal ones
-// have greater ids than k others.  After the first chunk, and each time the
-// row has grown `grow` times since, the block meets and, when the candidates
-// are half again as many as k, raises tau to about their k-th greatest and
-// drops the rest; in between its warps run on their own.  More candidates than the
+// maxima comes a value tau that at least k logits reach; what reaches it is a
+// candidate.  In later chunks only logits above tau can be alternatives, since
+// equal ones have greater ids than k others.  Each time the row has grown
+// `grow` times the block meets and, when the candidates are half again as
+// many as k, raises tau to about their k-th greatest and drops the rest; in
+// between its warps run on their own.  More candidates than the
 // buffer holds are cut out exactly: those of the first chunk from its staged
 // words (rows of few values, or masked but for fewer than k), those of a row
 // whose logits keep rising by reading it again.  What remains is ordered at
@@ -679,19 +750,19 @@ __device__ __noinline__ float cut_out(const Pool p, const Slice<E, NT> s, int w0
 // those that reach the least of the slices' about ceil(k / C)-th greatest are
 // at least k, and go to rank 0, which orders them.
 template <typename E, int NT, int D, bool TOPK, bool ENT>
-__global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreArgs a) {
+__global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(const ScoreArgs a) {
   constexpr int NW = NT / 32, kWide = kChunk * NT, kN = Word<E>::kN;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Stat part[2][NW];
   __shared__ Slip slip[2];
-  __shared__ float tau_s;
-  __shared__ int n_cand, n_ge, n_lead;
+  __shared__ float bound[2][NW], tau_s;
+  __shared__ int n_cand[2], n_ge, n_lead;
   uint4 *ring = reinterpret_cast<uint4 *>(smem);
-  // candidates, then (rank 0 of a cluster) those of all slices, then the first chunk's maxima
+  // candidates, then (rank 0 of a cluster) those of all slices
   unsigned long long *cand = reinterpret_cast<unsigned long long *>(smem + D * kWide * 16);
   unsigned long long *gath = cand + a.cap;
-  int *maxima = reinterpret_cast<int *>(gath + (a.in.C > 1 ? a.cap : 0));
-  const Pool pool = {cand, &n_cand, &n_ge, &tau_s, a.cap};
+  int par = 0;
+  auto pool = [&] { return Pool{cand, &n_cand[par], &n_ge, &tau_s, a.cap}; };
   const int t = threadIdx.x, lane = t & 31, wid = t >> 5;
   const int C = a.in.C;
   const unsigned rank = C > 1 ? cluster_ctarank() : 0;
@@ -724,7 +795,6 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
   };
   if (rank == 0 && wid * 32 < a.n_tok) next_tokens(r);
   for (int i = 0; i < D; ++i) send(ring + i * kWide);
-  int par = 0;
   for (; r < a.in.rows; par ^= 1) {
     // the tokens' logits, read beside the row's copies; the next row's tokens
     float zt[kMaxList / NT];
@@ -739,76 +809,84 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_score(const ScoreA
     }
     Running<E, ENT, false> run;
     float tau = -INFINITY, least = -INFINITY;  // of a chunk's logits, those from `least` on are candidates
-    int meet = 0;                              // the chunk after which the block meets next
+    int meet = a.grow - 1;                     // the chunk after which the block meets next
     for (int c = 0; c < chunks; ++c) {
       uint4 *at = ring + slot * kWide;
       slot = slot + 1 == D ? 0 : slot + 1;
       copies_wait<D - 1>();
       uint4 q[kChunk];
       cur.chunk(c, at, q);
-      const float cm = Word<E>::template max<kChunk>(q);
+      float wm[kChunk];
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) wm[j] = Word<E>::template max<1>(q + j);
+      const float cm = max_nan(max_nan(wm[0], wm[1]), max_nan(wm[2], wm[3]));
       run.add(q, cm, a.c, above);
       if (TOPK) {
         if (c == 0) {
-          // groups of four words (a thread's), two, or one
-          const int per = 4 * a.top_k <= NT ? 1 : 4 * a.top_k <= 2 * NT ? 2 : 4;
-          maxima[t] = ordered(per == 1 ? cm : Word<E>::template max<1>(q));
-          if (per == 2) {
-            maxima[t] = ordered(Word<E>::template max<2>(q));
-            maxima[NT + t] = ordered(Word<E>::template max<2>(q + 2));
-          } else if (per == 4) {
-#pragma unroll
-            for (int j = 1; j < kChunk; ++j) maxima[j * NT + t] = ordered(Word<E>::template max<1>(q + j));
+          // Each warp gives a value that its share of the k groups reach, of
+          // groups of four words, two, or one; all reach the least of these.
+          constexpr int kFew = 8;
+          const int k = (a.top_k + NW - 1) / NW;
+          float b;
+          if (k <= kFew) {
+            b = warp_kth<1>(&cm, k);
+          } else if (k <= 2 * kFew) {
+            const float v[2] = {max_nan(wm[0], wm[1]), max_nan(wm[2], wm[3])};
+            b = warp_kth<2>(v, k);
+          } else {
+            b = warp_kth<4>(wm, k);
           }
+          if (lane == 0) bound[par][wid] = b;
+          if (t == 0) n_cand[par] = 0;
           __syncthreads();
-          if (wid == 0) {
-            const float b = about_kth(maxima, 1, per * NT, a.top_k);
-            if (lane == 0) tau_s = b, n_cand = 0;
-          }
-          __syncthreads();
-          tau = least = tau_s;
+          tau = least = -warp_max_nan(-bound[par][lane % NW]);
         }
         if (cm >= least) {
           // this thread's hits as bits, room for them, then their keys
           unsigned hits = 0;
+          const unsigned lim = Word<E>::limit(least);
 #pragma unroll
-          for (int j = 0; j < kChunk; ++j) {
-            f2 v[kN / 2];
-            Word<E>::unpack(q[j], v);
-#pragma unroll
-            for (int k = 0; k < kN / 2; ++k) {
-              float x, y;
-              unpack2(v[k], x, y);
-              hits |= (x >= least ? 1u << (j * kN + 2 * k) : 0u) | (y >= least ? 2u << (j * kN + 2 * k) : 0u);
-            }
-          }
-          for (int p = atomicAdd(&n_cand, __popc(hits)); hits; hits &= hits - 1, ++p) {
+          for (int j = 0; j < kChunk; ++j)
+            if (wm[j] >= least) hits |= Word<E>::reach(q[j], lim) << (j * kN);
+          for (int p = atomicAdd(&n_cand[par], __popc(hits)); hits; hits &= hits - 1, ++p) {
             const int b = __ffs(hits) - 1, j = b / kN, k = b % kN, id = cur.id0(c * kWide + j * NT + t) + k;
             const float z = Word<E>::one(reinterpret_cast<const E *>(at + j * NT + t) + k);
             // the masked filling behind the row's ends is no logit: an empty key
             if (p < a.cap) cand[p] = id >= 0 && id < cur.V ? sort_key(z, id) : 0;
           }
         }
-        if (c == meet || c == chunks - 1) {
+        if (c + 1 < chunks && (c == meet || (c == 0 && tau == -INFINITY))) {
           __syncthreads();
-          const int n = n_cand;
+          const int n = n_cand[par];
           __syncthreads();
           if (n > a.cap)
-            tau = c == 0 ? cut_out<E, NT>(pool, cur, 0, kChunk, tau, a.top_k, a.soft, [at](int w) { return at[w]; })
-                         : cut_out<E, NT>(pool, cur, 0, (c + 1) * kChunk, tau, a.top_k, a.soft,
+            tau = c == 0 ? cut_out<E, NT>(pool(), cur, 0, kChunk, tau, a.top_k, a.soft, [at](int w) { return at[w]; })
+                         : cut_out<E, NT>(pool(), cur, 0, (c + 1) * kChunk, tau, a.top_k, a.soft,
                                           [cur](int w) { return cur.fetch(w); });
-          else if (n > a.soft && c < chunks - 1)
-            tau = thin_out<NT>(pool, n, a.top_k);
-          meet = a.grow * (meet + 1) - 1;
+          else if (n > a.soft)
+            tau = thin_out<NT>(pool(), n, a.top_k);
+          if (c == meet) meet = a.grow * (meet + 1) - 1;
         }
         least = next_up(tau);
       }
-      send(at);
+      if (c + 1 < chunks) send(at);
     }
     Stat st = combine_lanes<ENT, false>(run.get(), 32, a.c);
     if (lane == 0) part[par][wid] = st;
     __syncthreads();
-    const int n = TOPK ? n_cand : 0;
+    uint4 *last = ring + (slot == 0 ? D - 1 : slot - 1) * kWide;  // the row's last chunk, not yet sent for again
+    int n = TOPK ? n_cand[par] : 0;
+    if (TOPK && n > a.cap) {
+      if (chunks == 1)
+        cut_out<E, NT>(pool(), cur, 0, kChunk, tau, a.top_k, a.soft, [last](int w) { return last[w]; });
+      else
+        cut_out<E, NT>(pool(), cur, 0, chunks * kChunk, tau, a.top_k, a.soft, [cur](int w) { return cur.fetch(w); });
+      n = n_cand[par];
+    } else if (TOPK && n > 96 && n > 3 * a.top_k) {  // cheaper than ordering them all
+      thin_out<NT>(pool(), n, a.top_k);
+      n = n_cand[par];
+    }
+    send(last);
     if (C > 1) {
       if (wid == 0) {
         st = combine_lanes<ENT, false>(part[par][lane % NW], NW, a.c);
@@ -1385,13 +1463,13 @@ int row_words(const void *logits, int dtype, int vocab, long long ld) {
 // Streamed rows: a CTA a row, whatever its length.  When the rows leave SMs
 // short of CTAs a row is spread over a cluster of up to 8, down to slices of
 // 8 KB.
-Plan plan_stream(const void *logits, int dtype, int rows, int vocab, long long ld, int sms) {
+Plan plan_stream(const void *logits, int dtype, int rows, int vocab, long long ld, int top_k, int sms) {
   const int words = row_words(logits, dtype, vocab, ld);
   Plan p;
   p.C = 1;
   while (p.C < 8 && (long long)rows * p.C * 2 <= 2 * sms && words / (2 * p.C) >= 512) p.C *= 2;
   p.wps = (words + p.C - 1) / p.C;
-  p.nt = p.wps <= 1024 ? 128 : 256;
+  p.nt = p.wps <= 1024 || top_k <= 32 ? 128 : 256;
   p.even = ld * elem_size(dtype) % 16 == 0;
   return p;
 }
@@ -1472,7 +1550,7 @@ int by_dtype(int dtype, F &&f) {
   return f(__half());
 }
 
-constexpr int kRing128 = 4, kRing256 = 3;  // chunks in flight a CTA
+constexpr int kRing128 = 3, kRing256 = 4;  // chunks in flight a CTA
 
 template <typename E, int NT, int D>
 int score_nt(const char *who, const ScoreArgs &a, size_t smem, int dev, cudaStream_t st) {
@@ -1558,17 +1636,17 @@ int launch_score(const char *who, const ScoreLaunch &s, cudaStream_t stream) {
   a.entropy = s.entropy;
   a.top_ids = s.top_ids;
   a.top_logprob = s.top_logprob;
-  // A value that 1.25 k logits of a part of the row reach is reached by about
-  // 3.75 k more of four times as much: with room for 6 k the block meets each
+  // The first chunk's bound lets some 1.2 k to 2 k logits through and three
+  // times as many of the next three: with room for 10 k the block meets each
   // time the row has grown fourfold, else each time it has doubled.
   a.soft = s.top_k + s.top_k / 2 + 16;
-  for (a.cap = 256; a.cap < kMaxCap && a.cap < 6 * s.top_k;) a.cap *= 2;
-  a.grow = a.cap >= 6 * s.top_k ? 4 : 2;
-  const Plan p = plan_stream(s.logits, s.dtype, s.rows, s.V, s.ld, device_sm_count(dev));
+  for (a.cap = 512; a.cap < kMaxCap && a.cap < 10 * s.top_k;) a.cap *= 2;
+  a.grow = a.cap >= 10 * s.top_k ? 4 : 2;
+  const Plan p = plan_stream(s.logits, s.dtype, s.rows, s.V, s.ld, s.top_k, device_sm_count(dev));
   a.in.wps = p.wps;
   a.in.C = p.C;
   a.in.even = p.even;
-  const size_t lists = s.top_k ? (size_t)a.cap * 8 * (p.C > 1 ? 2 : 1) + (size_t)kChunk * p.nt * 4 : 0;
+  const size_t lists = s.top_k ? (size_t)a.cap * 8 * (p.C > 1 ? 2 : 1) : 0;
   const size_t smem = (size_t)(p.nt == 128 ? kRing128 : kRing256) * kChunk * p.nt * 16 + lists;
   return by_dtype(s.dtype, [&](auto e) {
     using E = decltype(e);
