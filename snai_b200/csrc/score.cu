@@ -456,8 +456,7 @@ __device__ __forceinline__ Stat no_stat() { return {-FLT_MAX, 0.f, 0.f, 0.f}; }
 // What a CTA tells the others of its cluster about its slice.
 struct __align__(16) Slip {
   Stat st;
-  double v[6];  // sums over the entries of a list (row gradients)
-  float tau;    // a bound of its alternatives (scores)
+  float tau;  // a bound of its alternatives (scores)
 };
 
 __device__ __forceinline__ Stat peer_stat(const Slip *mine, unsigned rank) {
@@ -988,48 +987,50 @@ struct RowGradArgs {
   long long grad_ld;
 };
 
+__device__ __forceinline__ void copy4(void *dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
 __device__ __forceinline__ double warp_sum_d(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// Sums over the entries of a row's list (see snai_row_grad).
-constexpr int kSums = 6;
-struct Entries {
-  double kl, qs;   // sum of q (log q - d), and of q, over the entries in the slice
-  double q;        // sum of q (MODE 0: of the token gradients) over the list
-  double se, se1;  // exponentials of the listed logits, at T and at temperature 1
-  double zy;       // the label's logit
-  __device__ __forceinline__ void add(const double *v) {
-    kl += v[0], qs += v[1], q += v[2], se += v[3], se1 += v[4], zy += v[5];
-  }
-  __device__ __forceinline__ void put(double *v) const {
-    v[0] = kl, v[1] = qs, v[2] = q, v[3] = se, v[4] = se1, v[5] = zy;
-  }
-  // over the warp
-  __device__ __forceinline__ void sum(bool rest, bool label1) {
-    kl = warp_sum_d(kl), qs = warp_sum_d(qs), q = warp_sum_d(q), zy = warp_sum_d(zy);
-    if (rest) se = warp_sum_d(se);
-    if (rest && label1) se1 = warp_sum_d(se1);
-  }
-};
-
-__device__ __forceinline__ void copy4(void *dst, const void *src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+// exp(x) in 64 bits for x <= 0 to about 1e-10: 2^n times the Taylor series
+// of exp over [-ln2 / 2, ln2 / 2] to the eighth power (0 below -700; a NaN
+// stays one, and what is not <= 0 by rounding or mistake is exact enough up
+// to 700).
+__device__ __forceinline__ double exp_d(double x) {
+  if (!(x > -700.0)) return x != x ? x : 0.0;
+  if (x > 700.0) return INFINITY;
+  const double n = rint(x * 1.4426950408889634074);
+  const double f = fma(-n, 0.69314718055994530942, x);
+  const double f2 = f * f;
+  const double lo = fma(f, fma(f, 1.0 / 6, 0.5), 1.0);                                    // 1 + f / 2 + f^2 / 6
+  const double hi = fma(f, fma(f, fma(f, fma(f, 1.0 / 40320, 1.0 / 5040), 1.0 / 720), 1.0 / 120), 1.0 / 24);
+  const double e = fma(f, fma(f2 * f, hi, lo), 1.0);
+  return e * __hiloint2double((1023 + (int)n) << 20, 0);
 }
 
-// first(j): no earlier entry of the list names the same id.
-__device__ __forceinline__ bool is_first(const int *ids, int j) {
+// Which of a list's n entries name the same id as entry j: an earlier one, a later one.
+__device__ __forceinline__ void same_ids(const int *ids, int n, int j, bool &earlier, bool &later) {
   const int id = ids[j];
   const int4 *v = reinterpret_cast<const int4 *>(ids);
-  bool seen = false;
-  int l = 0;
-  for (; l + 4 <= j; l += 4) {
+  earlier = later = false;
+#pragma unroll 2
+  for (int l = 0; l < n; l += 4) {  // the entries that fill up the last four are no ids
     const int4 x = v[l >> 2];
-    seen |= x.x == id || x.y == id || x.z == id || x.w == id;
+    const bool s[4] = {x.x == id, x.y == id, x.z == id, x.w == id};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) earlier |= s[k] && l + k < j, later |= s[k] && l + k > j && l + k < n;
   }
-  for (; l < j; ++l) seen |= ids[l] == id;
-  return !seen;
+}
+
+// Barrier of the cluster behind one thread's writes (the caller's thread 0,
+// which has fenced them): the other threads' gradient stores need not have
+// drained, as a release by every thread would have them.
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // MODE 0: the gradient of scores.  With x_i = d_i / ln 2, G the sum of the
@@ -1039,311 +1040,336 @@ __device__ __forceinline__ bool is_first(const int *ids, int j) {
 // MODE 1: distillation, q_j the teacher's weights:
 //   grad_i = e_i alpha + gamma softmax(z)_i - what the list and the label take.
 // EXTRA: labels at T != 1, whose softmax needs exponentials of its own.  With
-// `rest` the listed logits are taken out of the staged row, so that the
-// unlisted mass is a sum of its own (1 - the listed would lose a confident
-// student's); the list's part is summed separately.
-// Pass B writes the terms every element has; after a barrier the threads that
-// hold the entries write their ids' gradients.  An id listed more than once
-// is handled by its first entry, in the order of the list: no atomics.
-// The entries' weights and the loss are held in 64 bits: a handful of values
-// a row, and a loss that is a small difference of large terms.
+// `rest` the listed logits are taken out of the staged row (each by the thread
+// that owns its word, which finds it in a list of its own), so that the
+// unlisted mass is a sum of its own: 1 - the listed would lose a confident
+// student's.
+//
+// A row costs one barrier (`rest`: two).  Entry threads, which hold an entry
+// each, work their weights out while the row's words arrive, with the
+// entries' logits read from global memory; pass A ends in the barrier; every
+// warp then has the row's scalars and pass B writes the terms that every
+// element has.  The entries' ids get theirs one row later, behind the next
+// row's barrier, when all owners have written the base.  An id listed more
+// than once is handled by its first entry, in the order of the list: no
+// atomics.  The entries' weights and the loss are held in 64 bits: a handful
+// of values a row, and a loss that is a small difference of large terms.
 template <typename E, int NT, int MODE, bool EXTRA>
 __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_row_grad(const RowGradArgs a) {
-  constexpr int NW = NT / 32, kN = Word<E>::kN;
+  constexpr int NW = NT / 32, kN = Word<E>::kN, kWide = kChunk * NT;
   constexpr bool ENT = MODE == 0 && EXTRA, LABEL1 = MODE == 1 && EXTRA;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ Stat part[2][NW];
-  __shared__ float tch_m[NW], tch_s[NW];  // the teacher's list, by warp: maximum, sum of exponentials
-  __shared__ double sums[NW][kSums];
+  __shared__ Stat part[2][NW], listed[2][NW];
+  // by entry warp: the sums of q (MODE 0: g) and of q (log q - (z - top) / T), and top
+  __shared__ double sum_q[2][NW], sum_kl[2][NW];
+  __shared__ float list_top[2][NW];
+  __shared__ float label_z[2], scal[3];  // the label's logit; g_entropy or row_grad of three rows
   __shared__ Slip slip[2];
-  __shared__ float scal[2];  // g_entropy or row_grad of the row
   uint4 *buf = reinterpret_cast<uint4 *>(smem);
-  const bool rest = MODE == 1 && a.rest, soft = MODE == 1 && !a.rest;
+  const bool rest = MODE == 1 && a.rest;
   const int n = a.n, ne = n + (MODE == 1 && a.labels ? 1 : 0), cap = (ne + 3) & ~3;
-  // lists: ids and values of two rows, then weights and logits of this one
-  int *ids2 = reinterpret_cast<int *>(smem + (size_t)a.in.wps * 16);
-  float *vals2 = reinterpret_cast<float *>(ids2 + 2 * cap);
-  float *wt = vals2 + 2 * cap, *zl = wt + cap;
+  // lists: ids and values of three rows, weights of two; the entries' logits,
+  // pending gradients and links; heads of the owners' links
+  int *ids3 = reinterpret_cast<int *>(smem + (size_t)a.in.wps * 16);
+  float *vals3 = reinterpret_cast<float *>(ids3 + 3 * cap);
+  float *wt2 = vals3 + 3 * cap, *zl = wt2 + 2 * cap, *fix = zl + cap;
+  int *fix_id = reinterpret_cast<int *>(fix + cap), *link = fix_id + cap, *head = link + cap;
   const int t = threadIdx.x, lane = t & 31, wid = t >> 5;
   const int C = a.in.C;
   const unsigned rank = C > 1 ? cluster_ctarank() : 0;
   const int step = gridDim.x / C;
   const float above = kAbove / fmaxf(a.c, LABEL1 ? kLog2E : 0.f);
-  const int chunks = (a.in.wps + kChunk * NT - 1) / (kChunk * NT), cps = (chunks + kStages - 1) / kStages;
+  const int chunks = (a.in.wps + kWide - 1) / kWide, cps = (chunks + kStages - 1) / kStages;
   const int nwl = min((ne + 31) / 32, NW);  // warps that hold entries
+  const int V = a.in.V;
 
-  Slice<E, NT> cur, nxt;
-  int r = blockIdx.x / C, par = 0;
-  // a row's lists are committed with its first stage
-  auto load = [&](const Slice<E, NT> &s, int row, int p, int st) {
-    if (st == 0) {
-      for (int j = t; j < n; j += NT) {
-        copy4(ids2 + p * cap + j, a.ids + (long long)row * n + j);
-        copy4(vals2 + p * cap + j, a.vals + (long long)row * n + j);
-      }
-      if (ne > n && t == n % NT) copy4(ids2 + p * cap + n, a.labels + row);
-      if (t == 0) {
-        if (ENT) copy4(&scal[p], a.g_entropy + row);
-        if (MODE == 1 && a.row_grad) copy4(&scal[p], a.row_grad + row);
-      }
+  auto load_lists = [&](int row, int b) {
+    for (int j = t; j < n; j += NT) {
+      copy4(ids3 + b * cap + j, a.ids + (long long)row * n + j);
+      copy4(vals3 + b * cap + j, a.vals + (long long)row * n + j);
     }
+    if (ne > n && t == n % NT) copy4(ids3 + b * cap + n, a.labels + row);
+    if (t == 0) {
+      if (ENT) copy4(&scal[b], a.g_entropy + row);
+      if (MODE == 1 && a.row_grad) copy4(&scal[b], a.row_grad + row);
+    }
+  };
+  Slice<E, NT> cur, nxt;
+  int r = blockIdx.x / C, par = 0, b3 = 0;  // b3: the lists' place of this row
+  // stage st of `row`, with its first the lists of the row after it
+  auto load = [&](const Slice<E, NT> &s, int row, int b, int st) {
+    if (st == 0 && row + step < a.in.rows) load_lists(row + step, b);
     s.load(st, cps, buf);
   };
+  for (int j = t; j < 3 * cap; j += NT) ids3[j] = -1;
+  for (int j = t; j < ne; j += NT) fix_id[j] = -1;
+  if (rest) head[t] = -1;
+  __syncthreads();
+  load_lists(r, 0);
+  cur.commit();
   cur.set(a.in, r, rank);
-  for (int s = 0; s < kStages; ++s) load(cur, r, 0, s);
-  for (; r < a.in.rows; r += step, par ^= 1) {
+  for (int s = 0; s < kStages; ++s) load(cur, r, 1, s);
+  copies_wait<kStages>();
+  __syncthreads();
+  E *before = nullptr;  // the row whose entries' gradients are pending
+  for (; r < a.in.rows; r += step, par ^= 1, b3 = b3 == 2 ? 0 : b3 + 1) {
     const bool more = r + step < a.in.rows;
     nxt = cur;
     if (more) nxt.next(a.in, r, step, rank);
-    const int *ids = ids2 + par * cap;
-    const float *vals = vals2 + par * cap;
-    const int V = a.in.V;
+    const int after = b3 == 0 ? 2 : b3 - 1;  // the lists' place of the row after the next
+    const int *ids = ids3 + b3 * cap;
+    const float *vals = vals3 + b3 * cap;
+    float *wt = wt2 + par * cap;
     auto valid = [&](int id) { return id >= 0 && id < V; };
-    auto here = [&](int id) { return valid(id) && cur.local(id) >= 0; };  // in this slice
-    auto staged = [&](int id) { return reinterpret_cast<E *>(buf) + cur.local(id); };
-    bool any = false;  // anything but padding in the row?  (own entries, once they have landed)
-    auto look = [&] {
-      for (int j = t; j < ne; j += NT) any |= valid(ids[j]);
-      if (ENT && t == 0) any |= scal[par] != 0.f;
-    };
+    // the label, and g_entropy or row_grad: read now, for a call without a
+    // gradient sends for other lists before the barrier
+    const int y = ne > n && valid(ids[n]) ? ids[n] : -1;
+    const float sc = ENT || (MODE == 1 && a.row_grad) ? scal[b3] : 1.f;
+    bool any = ENT && t == 0 && sc != 0.f;  // anything but padding in the row?
+    unsigned firsts = 0, again = 0;               // by entry of this thread: the id's first; listed again later
+    if (wid < nwl) {
+      double lse = 0;
+      if (MODE == 1 && !rest) {  // the teacher's log normaliser, by every entry warp
+        float m = -INFINITY, s = 0.f;
+        for (int j = lane; j < n; j += 32)
+          if (valid(ids[j])) m = max_nan(m, vals[j]);
+        m = warp_max_nan(m);
+        for (int j = lane; j < n; j += 32)
+          if (valid(ids[j]) && vals[j] != -INFINITY) s += expf((vals[j] - m) * a.inv_t_f);
+        s = warp_sum(s);
+        lse = m == -INFINITY ? 0.0 : m * a.inv_t + (double)logf(s);
+      }
+      float top = -INFINITY;  // of the warp's listed logits
+      for (int j = t, i = 0; j < ne; j += NT, ++i) {
+        const int id = ids[j];
+        float z = -INFINITY;
+        if (valid(id)) {
+          z = load_now(cur.at(id));
+          bool earlier, later;
+          same_ids(ids, n, j, earlier, later);
+          firsts |= earlier ? 0u : 1u << i;
+          again |= later ? 1u << i : 0u;
+          any = true;
+        }
+        if (MODE == 1 && j == n)
+          label_z[par] = z;
+        else if (MODE == 1)
+          top = max_nan(top, z);
+        zl[j] = z;
+      }
+      // logits are taken relative to `top`, so that a row of the type's lowest values keeps its differences
+      top = MODE == 1 ? warp_max_nan(top) : 0.f;
+      if (top == -INFINITY) top = 0.f;
+      double q_own = 0, kl_own = 0;
+      Stat lst = no_stat();
+      for (int j = t, i = 0; j < n; j += NT, ++i) {
+        const int id = ids[j];
+        const float z = zl[j];
+        double q = 0;
+        if (MODE == 0) {
+          if (valid(id)) q = vals[j];
+        } else if (valid(id) && vals[j] != -INFINITY) {
+          const double lq = rest ? (double)vals[j] : vals[j] * a.inv_t - lse;
+          q = rest ? exp_d(lq) : (double)expf((float)lq);
+          if (q != 0.0) kl_own += q * (lq - ((double)z - top) * a.inv_t);
+        }
+        q_own += q;
+        wt[j] = (float)q;
+        if (rest && (firsts >> i & 1)) {
+          const float nm = max_nan(lst.m, z);
+          rebase<false, LABEL1>(lst, nm, a.c);
+          lst.s += ex2(cut((z - nm) * a.c));
+          if (LABEL1) lst.s1 += ex2(cut((z - nm) * kLog2E));
+          const int e = cur.local(id);
+          if (e >= 0) link[j] = atomicExch(&head[e / kN % NT], j);
+        }
+      }
+      if (ne > n && t == n % NT) wt[n] = 0.f;
+      q_own = warp_sum_d(q_own);
+      if (MODE == 1) kl_own = warp_sum_d(kl_own);
+      if (rest) lst = combine_lanes<false, LABEL1>(lst, 32, a.c);
+      if (lane == 0) {
+        sum_q[par][wid] = q_own;
+        if (MODE == 1) sum_kl[par][wid] = kl_own, list_top[par][wid] = top;
+        if (rest) listed[par][wid] = lst;
+      }
+    }
+    int mine = -1;  // the first of the listed logits in this thread's words
     if (rest) {
-      copies_wait<0>();
-      look();
-      any = __syncthreads_or(any);
-      for (int j = t; j < ne; j += NT)
-        if (here(ids[j])) zl[j] = Word<E>::one(staged(ids[j]));
       __syncthreads();
-      for (int j = t; j < n; j += NT)
-        if (here(ids[j])) Word<E>::put(staged(ids[j]), -INFINITY);
-      __syncthreads();
+      mine = head[t];
+      head[t] = -1;
     }
     // pass A
     Running<E, ENT, LABEL1> run;
     auto stage = [&](int s) {
       for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
+        for (int j = mine; j >= 0; j = link[j]) {
+          const int e = cur.local(ids[j]);
+          if (e / kN / kWide == c) Word<E>::put(reinterpret_cast<E *>(buf) + e, -INFINITY);
+        }
         uint4 q[kChunk];
-        cur.chunk(c, buf + c * cur.kWide, q);
+        cur.chunk(c, buf + c * kWide, q);
         run.add(q, Word<E>::template max<kChunk>(q), a.c, above);
       }
+      if (!a.grad && more) load(nxt, r + step, after, s);
     };
-    copies_wait<3>(), stage(0);
-    copies_wait<2>(), stage(1);
-    copies_wait<1>(), stage(2);
-    copies_wait<0>(), stage(3);
+    if (!a.grad && more) {  // no pass B: one group of the next row follows each stage
+      copies_wait<kStages - 1>(), stage(0);
+      copies_wait<kStages - 1>(), stage(1);
+      copies_wait<kStages - 1>(), stage(2);
+      copies_wait<kStages - 1>(), stage(3);
+    } else {
+      copies_wait<3>(), stage(0);
+      copies_wait<2>(), stage(1);
+      copies_wait<1>(), stage(2);
+      copies_wait<0>(), stage(3);
+    }
     Stat st = combine_lanes<ENT, LABEL1>(run.get(), 32, a.c);
     if (lane == 0) part[par][wid] = st;
-    if (soft && wid < nwl) {
-      float m = -INFINITY, s = 0.f;
-      for (int j = t; j < n; j += NT)
-        if (valid(ids[j])) m = max_nan(m, vals[j]);
-      m = warp_max_nan(m);
-      for (int j = t; j < n; j += NT)
-        if (valid(ids[j]) && vals[j] != -INFINITY) s += expf((vals[j] - m) * a.inv_t_f);
-      s = warp_sum(s);
-      if (lane == 0) tch_m[wid] = m, tch_s[wid] = s;
-    }
-    if (rest) {
-      __syncthreads();
-    } else {
-      look();
-      any = __syncthreads_or(any);
-    }
+    any = __syncthreads_or(any);
+    // the entries' gradients of the row before, over the base written by their words' owners
+    if (wid < nwl && before)
+      for (int j = t; j < ne; j += NT)
+        if (fix_id[j] >= 0) Word<E>::put(before + fix_id[j], fix[j]);
+    // the row's scalars, by every warp
     st = combine_lanes<ENT, LABEL1>(part[par][lane % NW], NW, a.c);
-    if (rest) {  // the listed logits may hold the slice's maximum
-      float m = -INFINITY;
-      for (int j = lane; j < n; j += 32)
-        if (here(ids[j])) m = max_nan(m, zl[j]);
-      rebase<ENT, LABEL1>(st, max_nan(st.m, warp_max_nan(m)), a.c);
-    }
-    // the entries' weights, and the sums over them
-    Entries own = {};
-    unsigned firsts = 0;
-    bool twice = false;
-    if (wid < nwl) {
-      double lse = 0;
-      if (soft) {
-        float m = -INFINITY, s = 0.f;
-        for (int w = 0; w < nwl; ++w) m = max_nan(m, tch_m[w]);
-        for (int w = 0; w < nwl; ++w)
-          if (tch_m[w] != -INFINITY) s += tch_s[w] * expf((tch_m[w] - m) * a.inv_t_f);
-        lse = m == -INFINITY ? 0.0 : m * a.inv_t + (double)logf(s);
-      }
-      for (int j = t, i = 0; j < ne; j += NT, ++i) {
-        const int id = ids[j];
-        const bool in = here(id);
-        if (in && !rest) zl[j] = Word<E>::one(staged(id));
-        if (valid(id)) {
-          if (is_first(ids, j))
-            firsts |= 1u << i;
-          else
-            twice = true;
-        }
-        double q = 0;
-        if (MODE == 1 && j == n) {
-          if (in) own.zy = zl[j];
-        } else if (MODE == 0) {
-          if (valid(id)) q = vals[j];
-        } else if (valid(id) && vals[j] != -INFINITY) {
-          const double lq = rest ? (double)vals[j] : vals[j] * a.inv_t - lse;
-          q = rest ? exp(lq) : (double)expf((float)lq);
-          if (in && q != 0.0) {
-            own.kl += q * (lq - ((double)zl[j] - st.m) * a.inv_t);
-            own.qs += q;
-          }
-        }
-        own.q += q;
-        if (rest && in && j < n && (firsts >> i & 1)) {
-          own.se += ex2(cut((zl[j] - st.m) * a.c));
-          if (LABEL1) own.se1 += ex2(cut((zl[j] - st.m) * kLog2E));
-        }
-        wt[j] = (float)q;
-      }
-      own.sum(rest, LABEL1);
-      if (lane == 0) own.put(sums[wid]);
-    }
-    const bool dups = __syncthreads_or(twice);
-    Entries tot = {};
-    for (int w = 0; w < nwl; ++w) tot.add(sums[w]);
     if (C > 1) {
       if (t == 0) {
         slip[par].st = st;
-        tot.put(slip[par].v);
+        fence_cluster();
       }
-      cluster_sync_all();
-      const double q_all = tot.q;  // every slice has seen the whole list
-      const Stat mine = lane % 16 < C ? peer_stat(&slip[par], lane % 16) : no_stat();
-      st = combine_lanes<ENT, LABEL1>(mine, 16, a.c);
-      tot = {};
-      if (lane < C) {
-        double v[kSums];
-        const uint32_t p = mapa_shared(smem_u32(slip[par].v), lane);
-        for (int k = 0; k < kSums; ++k) v[k] = ld_cluster_f64(p + 8 * k);
-        tot.add(v);
-        // d of the listed, and their exponentials, relative to the row's maximum
-        if (tot.qs > 0) tot.kl += tot.qs * (((double)st.m - mine.m) * a.inv_t);
-        tot.se *= ex2(cut((mine.m - st.m) * a.c));
-        tot.se1 *= ex2(cut((mine.m - st.m) * kLog2E));
-      }
-      tot.sum(rest, LABEL1);
-      tot.q = q_all;
+      __syncwarp();
+      cluster_meet();
+      st = combine_lanes<ENT, LABEL1>(lane % 16 < C ? peer_stat(&slip[par], lane % 16) : no_stat(), 16, a.c);
     }
-    // the row's scalars
-    const float S = rest ? st.s + (float)tot.se : st.s;
-    const float S1 = LABEL1 ? (rest ? st.s1 + (float)tot.se1 : st.s1) : S;
-    const float inv_s = S == 0.f ? 0.f : 1.f / S;
-    const int y = ne > n && valid(ids[n]) ? ids[n] : -1;
-    float alpha, beta = 0.f, gamma = 0.f, kt = 0.f, mass = 0.f, ru = 0.f, ky = 0.f;
+    double q_all = 0;
+    for (int w = 0; w < nwl; ++w) q_all += sum_q[par][w];
+    Stat lst = no_stat();
+    if (rest) {
+      if (lane % NW < nwl) lst = listed[par][lane % NW];
+      const float m = max_nan(st.m, warp_max_nan(lst.m));
+      rebase<false, LABEL1>(st, m, a.c);
+      rebase<false, LABEL1>(lst, m, a.c);
+      lst = combine_lanes<false, LABEL1>(lst, NW, a.c);
+    }
+    const float m = st.m, S = st.s + lst.s;
+    const float S1 = LABEL1 ? st.s1 + lst.s1 : S;
+    const float inv_s = S == 0.f ? 0.f : 1.f / S, inv_s1 = LABEL1 ? (S1 == 0.f ? 0.f : 1.f / S1) : inv_s;
+    float alpha, beta = 0.f, gamma = 0.f, kt = 0.f, ky = 0.f, mass = 0.f, ru = 0.f;
+    double rr = 0;
     if (MODE == 0) {
-      const float gh = ENT ? scal[par] : 0.f, k = inv_s * a.inv_t_f;
-      alpha = -(float)tot.q * k;
+      const float gh = ENT ? sc : 0.f, k = inv_s * a.inv_t_f;
+      alpha = -(float)q_all * k;
       if (ENT) alpha += gh * kLn2 * st.w * inv_s * k, beta = -gh * kLn2 * k;
     } else {
-      const double rr = rest && st.s > 0.f ? fmax(0.0, 1.0 - tot.q) : 0.0;
-      const float rg = a.row_grad ? scal[par] : 1.f;
-      mass = (float)(tot.q + rr);
+      rr = rest && st.s > 0.f ? fmax(0.0, 1.0 - q_all) : 0.0;
+      mass = (float)(q_all + rr);
       ru = rr > 0.0 ? (float)rr * (S / st.s) : 0.f;  // the teacher's rest over the student's
-      kt = rg * (float)((1.0 - a.a) * a.t);
-      ky = y >= 0 ? rg * (float)a.a : 0.f;
+      kt = sc * (float)((1.0 - a.a) * a.t);
+      ky = y >= 0 ? sc * (float)a.a : 0.f;
       alpha = kt * (mass - ru) * inv_s;
       if (LABEL1)
-        gamma = S1 == 0.f ? 0.f : ky / S1;
+        gamma = ky * inv_s1;
       else
         alpha += ky * inv_s;
-      if (t == 0 && rank == 0) {
-        double l = 0;
-        if (a.a < 1.0) {
-          l = S == 0.f ? (tot.q > 0 ? INFINITY : 0.0) : tot.kl + tot.q * log((double)S);
-          if (rr > 0.0) l += rr * (log(rr) + log1p(tot.se / st.s));
-          l *= (1.0 - a.a) * a.t * a.t;
-        }
-        if (y >= 0) l += a.a * (tot.zy == -INFINITY ? INFINITY : st.m - tot.zy + log((double)S1));
-        a.loss[r] = !any ? 0.f : S != S ? NAN : (float)l;
-      }
     }
-    if (!a.grad) {
-      if (more)
-        for (int s = 0; s < kStages; ++s) load(nxt, r + step, par ^ 1, s);
-      cur = nxt;
-      continue;
-    }
-    // pass B
-    E *out = static_cast<E *>(a.grad) + (long long)r * a.grad_ld;
-    const bool vec = ((reinterpret_cast<uintptr_t>(out) + (long long)cur.base * (int)sizeof(E)) & 15) == 0;
-    const f2 nm2 = pack2(-st.m, -st.m), c2 = pack2(a.c, a.c), l2 = pack2(kLog2E, kLog2E);
-    const f2 al2 = pack2(alpha, alpha), be2 = pack2(beta, beta), ga2 = pack2(gamma, gamma);
-#pragma unroll 1
-    for (int s = 0; s < kStages; ++s) {
-      for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
-        uint4 q[kChunk];
-        cur.chunk(c, buf + c * cur.kWide, q);
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-          f2 v[kN / 2];
-          Word<E>::unpack(q[j], v);
-#pragma unroll
-          for (int k = 0; k < kN / 2; ++k) {
-            const f2 d = add2(v[k], nm2);
-            f2 x = mul2(d, c2);
-            float u, w;
-            unpack2(x, u, w);
-            if (ENT) {
-              u = cut(u), w = cut(w);
-              x = pack2(u, w);
-            }
-            const f2 e = pack2(ex2(u), ex2(w));
-            v[k] = mul2(e, ENT ? fma2(x, be2, al2) : al2);
-            if (LABEL1) {
-              unpack2(mul2(d, l2), u, w);
-              v[k] = fma2(pack2(ex2(u), ex2(w)), ga2, v[k]);
-            }
-          }
-          q[j] = any ? Word<E>::pack(v) : make_uint4(0u, 0u, 0u, 0u);
-        }
-        const int w0 = c * cur.kWide + t;
-        E *o = out + cur.id0(w0);
-        if (vec && c * cur.kWide >= cur.lo && (c + 1) * cur.kWide <= cur.hi) {
-#pragma unroll
-          for (int j = 0; j < kChunk; ++j) *reinterpret_cast<uint4 *>(o + j * NT * kN) = q[j];
+    if (a.grad && wid < nwl)
+      for (int j = t, i = 0; j < ne; j += NT, ++i) {
+        const int id = ids[j];
+        fix_id[j] = any && (firsts >> i & 1) && cur.local(id) >= 0 ? id : -1;
+        float q = wt[j];
+        if (again >> i & 1)
+          for (int l = j + 1; l < n; ++l)
+            if (ids[l] == id) q += wt[l];
+        const float z = zl[j], d = z - m;
+        float g;
+        if (MODE == 0) {
+          const float x = cut(d * a.c);
+          g = ex2(x) * fmaf(x, beta, alpha) + q * a.inv_t_f;
         } else {
+          const float p = ex2(cut(d * a.c)) * inv_s;
+          g = kt * (j < n ? mass * p - q : (mass - ru) * p);
+          if (y >= 0) {
+            const float p1 = LABEL1 ? ex2(cut(d * kLog2E)) * inv_s1 : p;
+            g += ky * (id == y ? p1 - 1.f : p1);
+          }
+        }
+        fix[j] = S != S ? NAN : z == -INFINITY ? 0.f : g;
+      }
+    if (a.grad) {
+      // pass B
+      E *out = static_cast<E *>(a.grad) + (long long)r * a.grad_ld;
+      const bool vec = ((reinterpret_cast<uintptr_t>(out) + (long long)cur.base * (int)sizeof(E)) & 15) == 0;
+      const f2 nm2 = pack2(-m, -m), c2 = pack2(a.c, a.c), l2 = pack2(kLog2E, kLog2E);
+      const f2 al2 = pack2(alpha, alpha), be2 = pack2(beta, beta), ga2 = pack2(gamma, gamma);
+#pragma unroll 1
+      for (int s = 0; s < kStages; ++s) {
+#pragma unroll 1
+        for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
+          uint4 q[kChunk];
+          cur.chunk(c, buf + c * kWide, q);
 #pragma unroll
           for (int j = 0; j < kChunk; ++j) {
-            const int w = w0 + j * NT;
-            if (vec && w >= cur.lo && w < cur.hi)
-              *reinterpret_cast<uint4 *>(o + j * NT * kN) = q[j];
-            else if (w < cur.n)
-              cur.store_ragged(w, q[j], out);
+            f2 v[kN / 2];
+            Word<E>::unpack(q[j], v);
+#pragma unroll
+            for (int k = 0; k < kN / 2; ++k) {
+              const f2 d = add2(v[k], nm2);
+              f2 x = mul2(d, c2);
+              float u, w;
+              unpack2(x, u, w);
+              if (ENT) {
+                u = cut(u), w = cut(w);
+                x = pack2(u, w);
+              }
+              const f2 e = pack2(ex2(u), ex2(w));
+              v[k] = mul2(e, ENT ? fma2(x, be2, al2) : al2);
+              if (LABEL1) {
+                unpack2(mul2(d, l2), u, w);
+                v[k] = fma2(pack2(ex2(u), ex2(w)), ga2, v[k]);
+              }
+            }
+            q[j] = any ? Word<E>::pack(v) : make_uint4(0u, 0u, 0u, 0u);
           }
-        }
-      }
-      if (more) load(nxt, r + step, par ^ 1, s);
-    }
-    if (ne > 0) {
-      __syncthreads();  // the listed ids' gradients, over the base written by their words' owners
-      if (any)
-        for (int j = t, i = 0; j < ne; j += NT, ++i) {
-          const int id = ids[j];
-          if (!(firsts >> i & 1) || cur.local(id) < 0) continue;
-          float q = wt[j];
-          if (dups)
-            for (int l = j + 1; l < n; ++l)
-              if (ids[l] == id) q += wt[l];
-          const float z = zl[j], d = z - st.m;
-          float g;
-          if (MODE == 0) {
-            const float x = cut(d * a.c);
-            g = ex2(x) * fmaf(x, beta, alpha) + q * a.inv_t_f;
+          const int w0 = c * kWide + t;
+          E *o = out + cur.id0(w0);
+          if (vec && c * kWide >= cur.lo && (c + 1) * kWide <= cur.hi) {
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) *reinterpret_cast<uint4 *>(o + j * NT * kN) = q[j];
           } else {
-            const float p = ex2(cut(d * a.c)) * inv_s;
-            g = kt * (j < n ? mass * p - q : (mass - ru) * p);
-            if (y >= 0) {
-              const float p1 = LABEL1 ? ex2(cut(d * kLog2E)) / S1 : p;
-              g += ky * (id == y ? p1 - 1.f : p1);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) {
+              const int w = w0 + j * NT;
+              if (vec && w >= cur.lo && w < cur.hi)
+                *reinterpret_cast<uint4 *>(o + j * NT * kN) = q[j];
+              else if (w < cur.n)
+                cur.store_ragged(w, q[j], out);
             }
           }
-          Word<E>::put(out + id, S != S ? NAN : z == -INFINITY ? 0.f : g);
         }
+        if (more) load(nxt, r + step, after, s);
+      }
+      before = out;
+    }
+    if (MODE == 1 && t == NT - 32 && rank == 0) {  // the loss, by the last warp
+      double kl = 0, l = 0;
+      for (int w = 0; w < nwl; ++w) kl += sum_kl[par][w] + sum_q[par][w] * (((double)m - list_top[par][w]) * a.inv_t);
+      if (a.a < 1.0) {
+        l = S == 0.f ? (q_all > 0 ? INFINITY : 0.0) : kl + q_all * log((double)S);
+        if (rr > 0.0) l += rr * (log(rr) + log1p((double)lst.s / st.s));
+        l *= (1.0 - a.a) * a.t * a.t;
+      }
+      if (y >= 0) l += a.a * (label_z[par] == -INFINITY ? INFINITY : (double)m - label_z[par] + log((double)S1));
+      a.loss[r] = !any ? 0.f : S != S ? NAN : (float)l;
     }
     cur = nxt;
+  }
+  if (before) {
+    __syncthreads();
+    if (wid < nwl)
+      for (int j = t; j < ne; j += NT)
+        if (fix_id[j] >= 0) Word<E>::put(before + fix_id[j], fix[j]);
   }
   if (C > 1) cluster_sync_all();  // others may still read this CTA's slip
 }
@@ -1571,7 +1597,7 @@ int grad_nt(const char *who, const RowGradArgs &a, int mode, bool extra, size_t 
 
 int launch_row_grad(const char *who, RowGradArgs &a, int dtype, int mode, bool extra, int dev, cudaStream_t st) {
   const int ne = a.n + (a.labels ? 1 : 0);
-  const size_t lists = (size_t)((ne + 3) & ~3) * 6 * 4;
+  const size_t lists = (size_t)((ne + 3) & ~3) * 12 * 4 + 256 * 4;
   const Plan p = plan_staged(a.in.logits, dtype, a.in.rows, a.in.V, a.in.ld, lists, device_sm_count(dev));
   a.in.wps = p.wps;
   a.in.C = p.C;
