@@ -1011,18 +1011,20 @@ __device__ __forceinline__ double exp_d(double x) {
   return e * __hiloint2double((1023 + (int)n) << 20, 0);
 }
 
-// Which of a list's n entries name the same id as entry j: an earlier one, a later one.
+// Which of a list's n entries name the same id as entry j: an earlier one, a
+// later one.  (The entries that fill up the last four are no ids.)
 __device__ __forceinline__ void same_ids(const int *ids, int n, int j, bool &earlier, bool &later) {
   const int id = ids[j];
   const int4 *v = reinterpret_cast<const int4 *>(ids);
-  earlier = later = false;
-#pragma unroll 2
-  for (int l = 0; l < n; l += 4) {  // the entries that fill up the last four are no ids
+  int same = 0;
+#pragma unroll 4
+  for (int l = 0; l < n; l += 4) {
     const int4 x = v[l >> 2];
-    const bool s[4] = {x.x == id, x.y == id, x.z == id, x.w == id};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) earlier |= s[k] && l + k < j, later |= s[k] && l + k > j && l + k < n;
+    same += (x.x == id) + (x.y == id) + (x.z == id) + (x.w == id);
   }
+  earlier = later = false;
+  if (same > 1 || j >= n)  // j >= n: the label, behind the list
+    for (int l = 0; l < n; ++l) earlier |= l < j && ids[l] == id, later |= l > j && ids[l] == id;
 }
 
 // Barrier of the cluster behind one thread's writes (the caller's thread 0,
@@ -1045,102 +1047,143 @@ __device__ __forceinline__ void cluster_meet() {
 // unlisted mass is a sum of its own: 1 - the listed would lose a confident
 // student's.
 //
-// A row costs one barrier (`rest`: two).  Entry threads, which hold an entry
-// each, work their weights out while the row's words arrive, with the
-// entries' logits read from global memory; pass A ends in the barrier; every
-// warp then has the row's scalars and pass B writes the terms that every
-// element has.  The entries' ids get theirs one row later, behind the next
-// row's barrier, when all owners have written the base.  An id listed more
-// than once is handled by its first entry, in the order of the list: no
-// atomics.  The entries' weights and the loss are held in 64 bits: a handful
-// of values a row, and a loss that is a small difference of large terms.
+// The first NT threads stage the row and take it through both passes; 32 or
+// 64 more, the entry threads, have the list: they work a row ahead, with the
+// entries' logits read from global memory, so that what a row costs the others
+// is one barrier (`rest`: two) and the scalars, which every warp then works
+// out.  Pass B writes the terms that every element has; the entries' ids get
+// theirs from the entry threads one row later, behind the next row's barrier,
+// when all owners have written the base.  An id listed more than once is
+// handled by its first entry, in the order of the list: no atomics.  The
+// entries' weights and the loss are held in 64 bits: a handful of values a
+// row, and a loss that is a small difference of large terms.
+constexpr int kMaxEntryWarps = 2;
 template <typename E, int NT, int MODE, bool EXTRA>
-__global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_row_grad(const RowGradArgs a) {
+__global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) snai_row_grad(const RowGradArgs a) {
   constexpr int NW = NT / 32, kN = Word<E>::kN, kWide = kChunk * NT;
   constexpr bool ENT = MODE == 0 && EXTRA, LABEL1 = MODE == 1 && EXTRA;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ Stat part[2][NW], listed[2][NW];
+  __shared__ Stat part[2][NW], listed[2][kMaxEntryWarps];
   // by entry warp: the sums of q (MODE 0: g) and of q (log q - (z - top) / T), and top
-  __shared__ double sum_q[2][NW], sum_kl[2][NW];
-  __shared__ float list_top[2][NW];
-  __shared__ float label_z[2], scal[3];  // the label's logit; g_entropy or row_grad of three rows
+  __shared__ double sum_q[2][kMaxEntryWarps], sum_kl[kMaxEntryWarps];
+  __shared__ float list_top[kMaxEntryWarps];
+  __shared__ float label_z, scal[2];  // the label's logit; g_entropy or row_grad of two rows
   __shared__ Slip slip[2];
   uint4 *buf = reinterpret_cast<uint4 *>(smem);
   const bool rest = MODE == 1 && a.rest;
   const int n = a.n, ne = n + (MODE == 1 && a.labels ? 1 : 0), cap = (ne + 3) & ~3;
-  // lists: ids and values of three rows, weights of two; the entries' logits,
-  // pending gradients and links; heads of the owners' links
-  int *ids3 = reinterpret_cast<int *>(smem + (size_t)a.in.wps * 16);
-  float *vals3 = reinterpret_cast<float *>(ids3 + 3 * cap);
-  float *wt2 = vals3 + 3 * cap, *zl = wt2 + 2 * cap, *fix = zl + cap;
-  int *fix_id = reinterpret_cast<int *>(fix + cap), *link = fix_id + cap, *head = link + cap;
+  // lists: ids and values of two rows; the entries' weights and logits; the
+  // pending gradients; (rest) the owners' links, and their heads
+  int *ids2 = reinterpret_cast<int *>(smem + (size_t)a.in.wps * 16);
+  float *vals2 = reinterpret_cast<float *>(ids2 + 2 * cap);
+  float *wt = vals2 + 2 * cap, *zl = wt + cap, *fix = zl + cap;
+  int *fix_id = reinterpret_cast<int *>(fix + cap);
+  int2 *link = reinterpret_cast<int2 *>(fix_id + cap);
+  int *head = reinterpret_cast<int *>(link + cap);
   const int t = threadIdx.x, lane = t & 31, wid = t >> 5;
+  const bool entry = wid >= NW;
+  const int et = t - NT, ew = wid - NW, nwe = ((int)blockDim.x - NT) / 32, nte = nwe * 32;
   const int C = a.in.C;
   const unsigned rank = C > 1 ? cluster_ctarank() : 0;
   const int step = gridDim.x / C;
-  const float above = kAbove / fmaxf(a.c, LABEL1 ? kLog2E : 0.f);
-  const int chunks = (a.in.wps + kWide - 1) / kWide, cps = (chunks + kStages - 1) / kStages;
-  const int nwl = min((ne + 31) / 32, NW);  // warps that hold entries
   const int V = a.in.V;
-
+  auto valid = [&](int id) { return id >= 0 && id < V; };
   auto load_lists = [&](int row, int b) {
-    for (int j = t; j < n; j += NT) {
-      copy4(ids3 + b * cap + j, a.ids + (long long)row * n + j);
-      copy4(vals3 + b * cap + j, a.vals + (long long)row * n + j);
+    for (int j = et; j < n; j += nte) {
+      copy4(ids2 + b * cap + j, a.ids + (long long)row * n + j);
+      copy4(vals2 + b * cap + j, a.vals + (long long)row * n + j);
     }
-    if (ne > n && t == n % NT) copy4(ids3 + b * cap + n, a.labels + row);
-    if (t == 0) {
+    if (ne > n && et == n % nte) copy4(ids2 + b * cap + n, a.labels + row);
+    if (et == 0) {
       if (ENT) copy4(&scal[b], a.g_entropy + row);
       if (MODE == 1 && a.row_grad) copy4(&scal[b], a.row_grad + row);
     }
   };
-  Slice<E, NT> cur, nxt;
-  int r = blockIdx.x / C, par = 0, b3 = 0;  // b3: the lists' place of this row
-  // stage st of `row`, with its first the lists of the row after it
-  auto load = [&](const Slice<E, NT> &s, int row, int b, int st) {
-    if (st == 0 && row + step < a.in.rows) load_lists(row + step, b);
-    s.load(st, cps, buf);
-  };
-  for (int j = t; j < 3 * cap; j += NT) ids3[j] = -1;
-  for (int j = t; j < ne; j += NT) fix_id[j] = -1;
-  if (rest) head[t] = -1;
-  __syncthreads();
-  load_lists(r, 0);
-  cur.commit();
+  Slice<E, NT> cur;
+  int r = blockIdx.x / C;
   cur.set(a.in, r, rank);
-  for (int s = 0; s < kStages; ++s) load(cur, r, 1, s);
-  copies_wait<kStages>();
+  const int chunks = (a.in.wps + kWide - 1) / kWide, cps = (chunks + kStages - 1) / kStages;
+  if (entry) {
+    for (int j = et; j < cap; j += nte) ids2[cap + j] = fix_id[j] = -1;
+    for (int j = ne + et; j < cap; j += nte) ids2[j] = -1;
+    load_lists(r, 0);
+    cur.commit();
+    copies_wait<0>();
+  } else {
+    for (int s = 0; s < kStages; ++s) cur.load(s, cps, buf);
+    if (rest) head[t] = -1;
+  }
   __syncthreads();
-  E *before = nullptr;  // the row whose entries' gradients are pending
-  for (; r < a.in.rows; r += step, par ^= 1, b3 = b3 == 2 ? 0 : b3 + 1) {
-    const bool more = r + step < a.in.rows;
-    nxt = cur;
-    if (more) nxt.next(a.in, r, step, rank);
-    const int after = b3 == 0 ? 2 : b3 - 1;  // the lists' place of the row after the next
-    const int *ids = ids3 + b3 * cap;
-    const float *vals = vals3 + b3 * cap;
-    float *wt = wt2 + par * cap;
-    auto valid = [&](int id) { return id >= 0 && id < V; };
-    // the label, and g_entropy or row_grad: read now, for a call without a
-    // gradient sends for other lists before the barrier
-    const int y = ne > n && valid(ids[n]) ? ids[n] : -1;
-    const float sc = ENT || (MODE == 1 && a.row_grad) ? scal[b3] : 1.f;
-    bool any = ENT && t == 0 && sc != 0.f;  // anything but padding in the row?
-    unsigned firsts = 0, again = 0;               // by entry of this thread: the id's first; listed again later
-    if (wid < nwl) {
-      double lse = 0;
-      if (MODE == 1 && !rest) {  // the teacher's log normaliser, by every entry warp
-        float m = -INFINITY, s = 0.f;
-        for (int j = lane; j < n; j += 32)
-          if (valid(ids[j])) m = max_nan(m, vals[j]);
-        m = warp_max_nan(m);
-        for (int j = lane; j < n; j += 32)
-          if (valid(ids[j]) && vals[j] != -INFINITY) s += expf((vals[j] - m) * a.inv_t_f);
-        s = warp_sum(s);
-        lse = m == -INFINITY ? 0.0 : m * a.inv_t + (double)logf(s);
+  int par = 0;
+
+  // The scalars of a row, by every warp behind the row's barrier.
+  float m, S, S1, unlisted, inv_s, inv_s1, alpha, beta, gamma, kt, ky, mass, ru;
+  double rr, q_all;
+  Stat lst;
+  auto scalars = [&](float sc, int y) {
+    Stat st = combine_lanes<ENT, LABEL1>(part[par][lane % NW], NW, a.c);
+    if (C > 1) {
+      if (t == 0) {
+        slip[par].st = st;
+        fence_cluster();
       }
-      float top = -INFINITY;  // of the warp's listed logits
-      for (int j = t, i = 0; j < ne; j += NT, ++i) {
+      __syncwarp();
+      cluster_meet();
+      st = combine_lanes<ENT, LABEL1>(lane % 16 < C ? peer_stat(&slip[par], lane % 16) : no_stat(), 16, a.c);
+    }
+    q_all = sum_q[par][0];
+    if (nwe > 1) q_all += sum_q[par][1];
+    lst = no_stat();
+    if (rest) {
+      if (lane % 2 < nwe) lst = listed[par][lane % 2];
+      const float both = max_nan(st.m, warp_max_nan(lst.m));
+      rebase<false, LABEL1>(st, both, a.c);
+      rebase<false, LABEL1>(lst, both, a.c);
+      lst = combine_lanes<false, LABEL1>(lst, 2, a.c);
+    }
+    m = st.m;
+    S = st.s + lst.s;
+    S1 = LABEL1 ? st.s1 + lst.s1 : S;
+    inv_s = S == 0.f ? 0.f : 1.f / S;
+    inv_s1 = LABEL1 ? (S1 == 0.f ? 0.f : 1.f / S1) : inv_s;
+    unlisted = beta = gamma = kt = ky = mass = ru = 0.f;
+    rr = 0;
+    if (MODE == 0) {
+      const float gh = ENT ? sc : 0.f, k = inv_s * a.inv_t_f;
+      alpha = -(float)q_all * k;
+      if (ENT) alpha += gh * kLn2 * st.w * inv_s * k, beta = -gh * kLn2 * k;
+    } else {
+      rr = rest && st.s > 0.f ? fmax(0.0, 1.0 - q_all) : 0.0;
+      mass = (float)(q_all + rr);
+      unlisted = st.s;
+      ru = rr > 0.0 ? (float)rr * (S / st.s) : 0.f;  // the teacher's rest over the student's
+      kt = sc * (float)((1.0 - a.a) * a.t);
+      ky = y >= 0 ? sc * (float)a.a : 0.f;
+      alpha = kt * (mass - ru) * inv_s;
+      if (LABEL1)
+        gamma = ky * inv_s1;
+      else
+        alpha += ky * inv_s;
+    }
+  };
+
+  if (entry) {
+    E *before = nullptr;  // the row whose entries' gradients are pending
+    auto store_pending = [&] {
+      if (before)
+        for (int j = et; j < ne; j += nte)
+          if (fix_id[j] >= 0) Word<E>::put(before + fix_id[j], fix[j]);
+    };
+    for (; r < a.in.rows; r += step, par ^= 1) {
+      const int *ids = ids2 + par * cap;
+      const float *vals = vals2 + par * cap;
+      if (r + step < a.in.rows) load_lists(r + step, par ^ 1);
+      cur.commit();
+      const int y = ne > n && valid(ids[n]) ? ids[n] : -1;
+      const float sc = ENT || (MODE == 1 && a.row_grad) ? scal[par] : 1.f;
+      bool any = ENT && et == 0 && sc != 0.f;  // anything but padding in the row?
+      unsigned firsts = 0, again = 0;          // by entry of this thread: the id's first; listed again later
+      for (int j = et, i = 0; j < ne; j += nte, ++i) {
         const int id = ids[j];
         float z = -INFINITY;
         if (valid(id)) {
@@ -1150,19 +1193,34 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_row_grad(const Row
           firsts |= earlier ? 0u : 1u << i;
           again |= later ? 1u << i : 0u;
           any = true;
+          const int e = cur.local(id);
+          if (rest && !earlier && j < n && e >= 0) link[j] = make_int2(e, atomicExch(&head[e / kN % NT], j));
         }
-        if (MODE == 1 && j == n)
-          label_z[par] = z;
-        else if (MODE == 1)
-          top = max_nan(top, z);
         zl[j] = z;
       }
-      // logits are taken relative to `top`, so that a row of the type's lowest values keeps its differences
-      top = MODE == 1 ? warp_max_nan(top) : 0.f;
-      if (top == -INFINITY) top = 0.f;
+      if (rest) __syncthreads();  // the owners may take the links
+      double lse = 0;
+      if (MODE == 1 && !rest) {  // the teacher's log normaliser, by every entry warp
+        float tm = -INFINITY, s = 0.f;
+        for (int j = lane; j < n; j += 32)
+          if (valid(ids[j])) tm = max_nan(tm, vals[j]);
+        tm = warp_max_nan(tm);
+        for (int j = lane; j < n; j += 32)
+          if (valid(ids[j]) && vals[j] != -INFINITY) s += expf((vals[j] - tm) * a.inv_t_f);
+        s = warp_sum(s);
+        lse = tm == -INFINITY ? 0.0 : tm * a.inv_t + (double)logf(s);
+      }
+      // logits are taken relative to the warp's greatest, so that a row of the type's lowest values keeps its differences
+      float top = 0.f;
+      if (MODE == 1) {
+        top = -INFINITY;
+        for (int j = et; j < n; j += nte) top = max_nan(top, zl[j]);
+        top = warp_max_nan(top);
+        if (top == -INFINITY) top = 0.f;
+      }
       double q_own = 0, kl_own = 0;
-      Stat lst = no_stat();
-      for (int j = t, i = 0; j < n; j += NT, ++i) {
+      Stat own = no_stat();
+      for (int j = et, i = 0; j < n; j += nte, ++i) {
         const int id = ids[j];
         const float z = zl[j];
         double q = 0;
@@ -1176,200 +1234,189 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) snai_row_grad(const Row
         q_own += q;
         wt[j] = (float)q;
         if (rest && (firsts >> i & 1)) {
-          const float nm = max_nan(lst.m, z);
-          rebase<false, LABEL1>(lst, nm, a.c);
-          lst.s += ex2(cut((z - nm) * a.c));
-          if (LABEL1) lst.s1 += ex2(cut((z - nm) * kLog2E));
-          const int e = cur.local(id);
-          if (e >= 0) link[j] = atomicExch(&head[e / kN % NT], j);
+          const float nm = max_nan(own.m, z);
+          rebase<false, LABEL1>(own, nm, a.c);
+          own.s += ex2(cut((z - nm) * a.c));
+          if (LABEL1) own.s1 += ex2(cut((z - nm) * kLog2E));
         }
       }
-      if (ne > n && t == n % NT) wt[n] = 0.f;
-      q_own = warp_sum_d(q_own);
+      if (ne > n && et == n % nte) {
+        wt[n] = 0.f;
+        label_z = zl[n];
+      }
+      q_own = MODE == 0 ? (double)warp_sum((float)q_own) : warp_sum_d(q_own);
       if (MODE == 1) kl_own = warp_sum_d(kl_own);
-      if (rest) lst = combine_lanes<false, LABEL1>(lst, 32, a.c);
+      if (rest) own = combine_lanes<false, LABEL1>(own, 32, a.c);
       if (lane == 0) {
-        sum_q[par][wid] = q_own;
-        if (MODE == 1) sum_kl[par][wid] = kl_own, list_top[par][wid] = top;
-        if (rest) listed[par][wid] = lst;
+        sum_q[par][ew] = q_own;
+        if (MODE == 1) sum_kl[ew] = kl_own, list_top[ew] = top;
+        if (rest) listed[par][ew] = own;
       }
-    }
-    int mine = -1;  // the first of the listed logits in this thread's words
-    if (rest) {
-      __syncthreads();
-      mine = head[t];
-      head[t] = -1;
-    }
-    // pass A
-    Running<E, ENT, LABEL1> run;
-    auto stage = [&](int s) {
-      for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
-        for (int j = mine; j >= 0; j = link[j]) {
-          const int e = cur.local(ids[j]);
-          if (e / kN / kWide == c) Word<E>::put(reinterpret_cast<E *>(buf) + e, -INFINITY);
-        }
-        uint4 q[kChunk];
-        cur.chunk(c, buf + c * kWide, q);
-        run.add(q, Word<E>::template max<kChunk>(q), a.c, above);
-      }
-      if (!a.grad && more) load(nxt, r + step, after, s);
-    };
-    if (!a.grad && more) {  // no pass B: one group of the next row follows each stage
-      copies_wait<kStages - 1>(), stage(0);
-      copies_wait<kStages - 1>(), stage(1);
-      copies_wait<kStages - 1>(), stage(2);
-      copies_wait<kStages - 1>(), stage(3);
-    } else {
-      copies_wait<3>(), stage(0);
-      copies_wait<2>(), stage(1);
-      copies_wait<1>(), stage(2);
-      copies_wait<0>(), stage(3);
-    }
-    Stat st = combine_lanes<ENT, LABEL1>(run.get(), 32, a.c);
-    if (lane == 0) part[par][wid] = st;
-    any = __syncthreads_or(any);
-    // the entries' gradients of the row before, over the base written by their words' owners
-    if (wid < nwl && before)
-      for (int j = t; j < ne; j += NT)
-        if (fix_id[j] >= 0) Word<E>::put(before + fix_id[j], fix[j]);
-    // the row's scalars, by every warp
-    st = combine_lanes<ENT, LABEL1>(part[par][lane % NW], NW, a.c);
-    if (C > 1) {
-      if (t == 0) {
-        slip[par].st = st;
-        fence_cluster();
-      }
-      __syncwarp();
-      cluster_meet();
-      st = combine_lanes<ENT, LABEL1>(lane % 16 < C ? peer_stat(&slip[par], lane % 16) : no_stat(), 16, a.c);
-    }
-    double q_all = 0;
-    for (int w = 0; w < nwl; ++w) q_all += sum_q[par][w];
-    Stat lst = no_stat();
-    if (rest) {
-      if (lane % NW < nwl) lst = listed[par][lane % NW];
-      const float m = max_nan(st.m, warp_max_nan(lst.m));
-      rebase<false, LABEL1>(st, m, a.c);
-      rebase<false, LABEL1>(lst, m, a.c);
-      lst = combine_lanes<false, LABEL1>(lst, NW, a.c);
-    }
-    const float m = st.m, S = st.s + lst.s;
-    const float S1 = LABEL1 ? st.s1 + lst.s1 : S;
-    const float inv_s = S == 0.f ? 0.f : 1.f / S, inv_s1 = LABEL1 ? (S1 == 0.f ? 0.f : 1.f / S1) : inv_s;
-    float alpha, beta = 0.f, gamma = 0.f, kt = 0.f, ky = 0.f, mass = 0.f, ru = 0.f;
-    double rr = 0;
-    if (MODE == 0) {
-      const float gh = ENT ? sc : 0.f, k = inv_s * a.inv_t_f;
-      alpha = -(float)q_all * k;
-      if (ENT) alpha += gh * kLn2 * st.w * inv_s * k, beta = -gh * kLn2 * k;
-    } else {
-      rr = rest && st.s > 0.f ? fmax(0.0, 1.0 - q_all) : 0.0;
-      mass = (float)(q_all + rr);
-      ru = rr > 0.0 ? (float)rr * (S / st.s) : 0.f;  // the teacher's rest over the student's
-      kt = sc * (float)((1.0 - a.a) * a.t);
-      ky = y >= 0 ? sc * (float)a.a : 0.f;
-      alpha = kt * (mass - ru) * inv_s;
-      if (LABEL1)
-        gamma = ky * inv_s1;
-      else
-        alpha += ky * inv_s;
-    }
-    if (a.grad && wid < nwl)
-      for (int j = t, i = 0; j < ne; j += NT, ++i) {
-        const int id = ids[j];
-        fix_id[j] = any && (firsts >> i & 1) && cur.local(id) >= 0 ? id : -1;
-        float q = wt[j];
-        if (again >> i & 1)
-          for (int l = j + 1; l < n; ++l)
-            if (ids[l] == id) q += wt[l];
-        const float z = zl[j], d = z - m;
-        float g;
-        if (MODE == 0) {
-          const float x = cut(d * a.c);
-          g = ex2(x) * fmaf(x, beta, alpha) + q * a.inv_t_f;
-        } else {
-          const float p = ex2(cut(d * a.c)) * inv_s;
-          g = kt * (j < n ? mass * p - q : (mass - ru) * p);
-          if (y >= 0) {
-            const float p1 = LABEL1 ? ex2(cut(d * kLog2E)) * inv_s1 : p;
-            g += ky * (id == y ? p1 - 1.f : p1);
+      copies_wait<0>();  // the next row's lists
+      any = __syncthreads_or(any);
+      store_pending();  // over the base that the row before's owners have written
+      scalars(sc, y);
+      if (a.grad) {
+        for (int j = et, i = 0; j < ne; j += nte, ++i) {
+          const int id = ids[j];
+          fix_id[j] = any && (firsts >> i & 1) && cur.local(id) >= 0 ? id : -1;
+          float q = wt[j];
+          if (again >> i & 1)
+            for (int l = j + 1; l < n; ++l)
+              if (ids[l] == id) q += wt[l];
+          const float z = zl[j], d = z - m;
+          float g;
+          if (MODE == 0) {
+            const float x = cut(d * a.c);
+            g = ex2(x) * fmaf(x, beta, alpha) + q * a.inv_t_f;
+          } else {
+            const float p = ex2(cut(d * a.c)) * inv_s;
+            g = kt * (j < n ? mass * p - q : (mass - ru) * p);
+            if (y >= 0) {
+              const float p1 = LABEL1 ? ex2(cut(d * kLog2E)) * inv_s1 : p;
+              g += ky * (id == y ? p1 - 1.f : p1);
+            }
           }
+          fix[j] = S != S ? NAN : z == -INFINITY ? 0.f : g;
         }
-        fix[j] = S != S ? NAN : z == -INFINITY ? 0.f : g;
+        before = static_cast<E *>(a.grad) + (long long)r * a.grad_ld;
       }
-    if (a.grad) {
-      // pass B
-      E *out = static_cast<E *>(a.grad) + (long long)r * a.grad_ld;
-      const bool vec = ((reinterpret_cast<uintptr_t>(out) + (long long)cur.base * (int)sizeof(E)) & 15) == 0;
-      const f2 nm2 = pack2(-m, -m), c2 = pack2(a.c, a.c), l2 = pack2(kLog2E, kLog2E);
-      const f2 al2 = pack2(alpha, alpha), be2 = pack2(beta, beta), ga2 = pack2(gamma, gamma);
-#pragma unroll 1
-      for (int s = 0; s < kStages; ++s) {
-#pragma unroll 1
+      if (MODE == 1 && et == 0 && rank == 0) {
+        double l = 0;
+        if (a.a < 1.0) {
+          if (S == 0.f) {
+            l = q_all > 0 ? INFINITY : 0.0;
+          } else {
+            for (int w = 0; w < nwe; ++w) l += sum_kl[w] + sum_q[par][w] * (((double)m - list_top[w]) * a.inv_t);
+            l += q_all * log((double)S);
+            if (rr > 0.0) l += rr * (log(rr) + log1p((double)lst.s / unlisted));
+          }
+          l *= (1.0 - a.a) * a.t * a.t;
+        }
+        if (y >= 0) l += a.a * (label_z == -INFINITY ? INFINITY : (double)m - label_z + log((double)S1));
+        a.loss[r] = !any ? 0.f : S != S ? NAN : (float)l;
+      }
+      // what the entry warps share of a row (weights, sums, the label's logit) is overwritten by the next
+      if (nwe > 1)
+        asm volatile("bar.sync 1, %0;" ::"r"(nte) : "memory");
+      else
+        __syncwarp();
+      if (r + step < a.in.rows) cur.next(a.in, r, step, rank);
+    }
+    __syncthreads();
+    store_pending();
+  } else {
+    const float above = kAbove / fmaxf(a.c, LABEL1 ? kLog2E : 0.f);
+    for (; r < a.in.rows; r += step, par ^= 1) {
+      const bool more = r + step < a.in.rows;
+      Slice<E, NT> nxt = cur;
+      if (more) nxt.next(a.in, r, step, rank);
+      const int label = ne > n ? ids2[par * cap + n] : -1, y = valid(label) ? label : -1;
+      const float sc = ENT || (MODE == 1 && a.row_grad) ? scal[par] : 1.f;
+      // the listed logits among this thread's words: two at hand, the others linked
+      int e0 = -1, e1 = -1, others = -1;
+      if (rest) {
+        __syncthreads();
+        others = head[t];
+        if (others >= 0) {
+          head[t] = -1;
+          int2 l = link[others];
+          e0 = l.x, others = l.y;
+          if (others >= 0) l = link[others], e1 = l.x, others = l.y;
+        }
+      }
+      const int c0 = e0 < 0 ? -1 : e0 / (kN * kWide), c1 = e1 < 0 ? -1 : e1 / (kN * kWide);
+      // pass A
+      Running<E, ENT, LABEL1> run;
+      auto stage = [&](int s) {
         for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
+          if (rest) {
+            if (c0 == c) Word<E>::put(reinterpret_cast<E *>(buf) + e0, -INFINITY);
+            if (c1 == c) Word<E>::put(reinterpret_cast<E *>(buf) + e1, -INFINITY);
+            for (int j = others; j >= 0;) {
+              const int2 l = link[j];
+              if (l.x / (kN * kWide) == c) Word<E>::put(reinterpret_cast<E *>(buf) + l.x, -INFINITY);
+              j = l.y;
+            }
+          }
           uint4 q[kChunk];
           cur.chunk(c, buf + c * kWide, q);
-#pragma unroll
-          for (int j = 0; j < kChunk; ++j) {
-            f2 v[kN / 2];
-            Word<E>::unpack(q[j], v);
-#pragma unroll
-            for (int k = 0; k < kN / 2; ++k) {
-              const f2 d = add2(v[k], nm2);
-              f2 x = mul2(d, c2);
-              float u, w;
-              unpack2(x, u, w);
-              if (ENT) {
-                u = cut(u), w = cut(w);
-                x = pack2(u, w);
-              }
-              const f2 e = pack2(ex2(u), ex2(w));
-              v[k] = mul2(e, ENT ? fma2(x, be2, al2) : al2);
-              if (LABEL1) {
-                unpack2(mul2(d, l2), u, w);
-                v[k] = fma2(pack2(ex2(u), ex2(w)), ga2, v[k]);
-              }
-            }
-            q[j] = any ? Word<E>::pack(v) : make_uint4(0u, 0u, 0u, 0u);
-          }
-          const int w0 = c * kWide + t;
-          E *o = out + cur.id0(w0);
-          if (vec && c * kWide >= cur.lo && (c + 1) * kWide <= cur.hi) {
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) *reinterpret_cast<uint4 *>(o + j * NT * kN) = q[j];
-          } else {
+          run.add(q, Word<E>::template max<kChunk>(q), a.c, above);
+        }
+        if (!a.grad && more) nxt.load(s, cps, buf);
+      };
+      if (!a.grad && more) {  // no pass B: one group of the next row follows each stage
+        copies_wait<kStages - 1>(), stage(0);
+        copies_wait<kStages - 1>(), stage(1);
+        copies_wait<kStages - 1>(), stage(2);
+        copies_wait<kStages - 1>(), stage(3);
+      } else {
+        copies_wait<3>(), stage(0);
+        copies_wait<2>(), stage(1);
+        copies_wait<1>(), stage(2);
+        copies_wait<0>(), stage(3);
+      }
+      const Stat st = combine_lanes<ENT, LABEL1>(run.get(), 32, a.c);
+      if (lane == 0) part[par][wid] = st;
+      const bool any = __syncthreads_or(false);
+      if (a.grad || C > 1) scalars(sc, y);
+      if (a.grad) {
+        // pass B
+        E *out = static_cast<E *>(a.grad) + (long long)r * a.grad_ld;
+        const bool vec = ((reinterpret_cast<uintptr_t>(out) + (long long)cur.base * (int)sizeof(E)) & 15) == 0;
+        const f2 nm2 = pack2(-m, -m), c2 = pack2(a.c, a.c), l2 = pack2(kLog2E, kLog2E);
+        const f2 al2 = pack2(alpha, alpha), be2 = pack2(beta, beta), ga2 = pack2(gamma, gamma);
+#pragma unroll 1
+        for (int s = 0; s < kStages; ++s) {
+#pragma unroll 1
+          for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
+            uint4 q[kChunk];
+            cur.chunk(c, buf + c * kWide, q);
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
-              const int w = w0 + j * NT;
-              if (vec && w >= cur.lo && w < cur.hi)
-                *reinterpret_cast<uint4 *>(o + j * NT * kN) = q[j];
-              else if (w < cur.n)
-                cur.store_ragged(w, q[j], out);
+              f2 v[kN / 2];
+              Word<E>::unpack(q[j], v);
+#pragma unroll
+              for (int k = 0; k < kN / 2; ++k) {
+                const f2 d = add2(v[k], nm2);
+                f2 x = mul2(d, c2);
+                float u, w;
+                unpack2(x, u, w);
+                if (ENT) {
+                  u = cut(u), w = cut(w);
+                  x = pack2(u, w);
+                }
+                const f2 e = pack2(ex2(u), ex2(w));
+                v[k] = mul2(e, ENT ? fma2(x, be2, al2) : al2);
+                if (LABEL1) {
+                  unpack2(mul2(d, l2), u, w);
+                  v[k] = fma2(pack2(ex2(u), ex2(w)), ga2, v[k]);
+                }
+              }
+              q[j] = any ? Word<E>::pack(v) : make_uint4(0u, 0u, 0u, 0u);
+            }
+            const int w0 = c * kWide + t;
+            E *o = out + cur.id0(w0);
+            if (vec && c * kWide >= cur.lo && (c + 1) * kWide <= cur.hi) {
+#pragma unroll
+              for (int j = 0; j < kChunk; ++j) *reinterpret_cast<uint4 *>(o + j * NT * kN) = q[j];
+            } else {
+#pragma unroll
+              for (int j = 0; j < kChunk; ++j) {
+                const int w = w0 + j * NT;
+                if (vec && w >= cur.lo && w < cur.hi)
+                  *reinterpret_cast<uint4 *>(o + j * NT * kN) = q[j];
+                else if (w < cur.n)
+                  cur.store_ragged(w, q[j], out);
+              }
             }
           }
+          if (more) nxt.load(s, cps, buf);
         }
-        if (more) load(nxt, r + step, after, s);
       }
-      before = out;
+      cur = nxt;
     }
-    if (MODE == 1 && t == NT - 32 && rank == 0) {  // the loss, by the last warp
-      double kl = 0, l = 0;
-      for (int w = 0; w < nwl; ++w) kl += sum_kl[par][w] + sum_q[par][w] * (((double)m - list_top[par][w]) * a.inv_t);
-      if (a.a < 1.0) {
-        l = S == 0.f ? (q_all > 0 ? INFINITY : 0.0) : kl + q_all * log((double)S);
-        if (rr > 0.0) l += rr * (log(rr) + log1p((double)lst.s / st.s));
-        l *= (1.0 - a.a) * a.t * a.t;
-      }
-      if (y >= 0) l += a.a * (label_z[par] == -INFINITY ? INFINITY : (double)m - label_z[par] + log((double)S1));
-      a.loss[r] = !any ? 0.f : S != S ? NAN : (float)l;
-    }
-    cur = nxt;
-  }
-  if (before) {
     __syncthreads();
-    if (wid < nwl)
-      for (int j = t; j < ne; j += NT)
-        if (fix_id[j] >= 0) Word<E>::put(before + fix_id[j], fix[j]);
   }
   if (C > 1) cluster_sync_all();  // others may still read this CTA's slip
 }
@@ -1538,11 +1585,11 @@ int launch_rows(const char *who, void (*kern)(A), const A &args, int nt, size_t 
   cfg.numAttrs = C > 1 ? 1 : 0;
   cfg.gridDim = dim3((unsigned)C);
   static std::mutex mu;
-  static std::map<std::tuple<const void *, int, int, size_t>, int> fits;
+  static std::map<std::tuple<const void *, int, int, int, size_t>, int> fits;
   int fit = 0;
   {
     std::lock_guard<std::mutex> g(mu);
-    int &f = fits[std::make_tuple(fn, dev, C, smem)];
+    int &f = fits[std::make_tuple(fn, dev, C, nt, smem)];
     if (f == 0) {
       bool ok = set_dyn_smem(kern, 227 * 1024);
       ok = ok && cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, 100) == cudaSuccess;
@@ -1587,17 +1634,20 @@ int score_nt(const char *who, const ScoreArgs &a, size_t smem, int dev, cudaStre
 
 // mode 0: scores' gradient, 1: distillation; extra: as the kernel's EXTRA
 template <typename E, int NT>
-int grad_nt(const char *who, const RowGradArgs &a, int mode, bool extra, size_t smem, int dev, cudaStream_t st) {
+int grad_nt(const char *who, const RowGradArgs &a, int mode, bool extra, int entry, size_t smem, int dev,
+            cudaStream_t st) {
+  const int nt = NT + entry;
   if (mode == 0)
-    return extra ? launch_rows(who, snai_row_grad<E, NT, 0, true>, a, NT, smem, dev, st)
-                 : launch_rows(who, snai_row_grad<E, NT, 0, false>, a, NT, smem, dev, st);
-  return extra ? launch_rows(who, snai_row_grad<E, NT, 1, true>, a, NT, smem, dev, st)
-               : launch_rows(who, snai_row_grad<E, NT, 1, false>, a, NT, smem, dev, st);
+    return extra ? launch_rows(who, snai_row_grad<E, NT, 0, true>, a, nt, smem, dev, st)
+                 : launch_rows(who, snai_row_grad<E, NT, 0, false>, a, nt, smem, dev, st);
+  return extra ? launch_rows(who, snai_row_grad<E, NT, 1, true>, a, nt, smem, dev, st)
+               : launch_rows(who, snai_row_grad<E, NT, 1, false>, a, nt, smem, dev, st);
 }
 
 int launch_row_grad(const char *who, RowGradArgs &a, int dtype, int mode, bool extra, int dev, cudaStream_t st) {
   const int ne = a.n + (a.labels ? 1 : 0);
-  const size_t lists = (size_t)((ne + 3) & ~3) * 12 * 4 + 256 * 4;
+  const size_t lists = (size_t)((ne + 3) & ~3) * 10 * 4 + 256 * 4;
+  const int entry = ne > 32 ? 64 : 32;  // entry threads
   const Plan p = plan_staged(a.in.logits, dtype, a.in.rows, a.in.V, a.in.ld, lists, device_sm_count(dev));
   a.in.wps = p.wps;
   a.in.C = p.C;
@@ -1605,8 +1655,8 @@ int launch_row_grad(const char *who, RowGradArgs &a, int dtype, int mode, bool e
   const size_t smem = (size_t)p.wps * 16 + lists;
   return by_dtype(dtype, [&](auto e) {
     using E = decltype(e);
-    return p.nt == 128 ? grad_nt<E, 128>(who, a, mode, extra, smem, dev, st)
-                       : grad_nt<E, 256>(who, a, mode, extra, smem, dev, st);
+    return p.nt == 128 ? grad_nt<E, 128>(who, a, mode, extra, entry, smem, dev, st)
+                       : grad_nt<E, 256>(who, a, mode, extra, entry, smem, dev, st);
   });
 }
 
