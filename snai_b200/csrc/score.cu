@@ -367,6 +367,16 @@ struct Slice {
 template <int N> __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+__device__ __forceinline__ void copies_wait(int n) {  // n < kStages
+  if (n == 0)
+    copies_wait<0>();
+  else if (n == 1)
+    copies_wait<1>();
+  else if (n == 2)
+    copies_wait<2>();
+  else
+    copies_wait<3>();
+}
 
 // ---- softmax statistics ----
 
@@ -1185,20 +1195,18 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
       unsigned firsts = 0, again = 0;          // by entry of this thread: the id's first; listed again later
       for (int j = et, i = 0; j < ne; j += nte, ++i) {
         const int id = ids[j];
-        float z = -INFINITY;
-        if (valid(id)) {
-          z = load_now(cur.at(id));
-          bool earlier, later;
-          same_ids(ids, n, j, earlier, later);
-          firsts |= earlier ? 0u : 1u << i;
-          again |= later ? 1u << i : 0u;
-          any = true;
-          const int e = cur.local(id);
-          if (rest && !earlier && j < n && e >= 0) link[j] = make_int2(e, atomicExch(&head[e / kN % NT], j));
-        }
-        zl[j] = z;
+        if (!valid(id)) continue;
+        bool earlier, later;
+        same_ids(ids, n, j, earlier, later);
+        firsts |= earlier ? 0u : 1u << i;
+        again |= later ? 1u << i : 0u;
+        any = true;
+        const int e = cur.local(id);
+        if (rest && !earlier && j < n && e >= 0) link[j] = make_int2(e, atomicExch(&head[e / kN % NT], j));
       }
       if (rest) __syncthreads();  // the owners may take the links
+#pragma unroll 2
+      for (int j = et; j < ne; j += nte) zl[j] = valid(ids[j]) ? Word<E>::one(cur.at(ids[j])) : -INFINITY;
       double lse = 0;
       if (MODE == 1 && !rest) {  // the teacher's log normaliser, by every entry warp
         float tm = -INFINITY, s = 0.f;
@@ -1328,7 +1336,13 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
       const int c0 = e0 < 0 ? -1 : e0 / (kN * kWide), c1 = e1 < 0 ? -1 : e1 / (kN * kWide);
       // pass A
       Running<E, ENT, LABEL1> run;
-      auto stage = [&](int s) {
+#pragma unroll 1
+      for (int s = 0; s < kStages; ++s) {
+        if (!a.grad && more)  // no pass B: one group of the next row follows each stage
+          copies_wait<kStages - 1>();
+        else
+          copies_wait(kStages - 1 - s);
+#pragma unroll 1
         for (int c = s * cps; c < (s + 1) * cps && c < chunks; ++c) {
           if (rest) {
             if (c0 == c) Word<E>::put(reinterpret_cast<E *>(buf) + e0, -INFINITY);
@@ -1344,17 +1358,6 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
           run.add(q, Word<E>::template max<kChunk>(q), a.c, above);
         }
         if (!a.grad && more) nxt.load(s, cps, buf);
-      };
-      if (!a.grad && more) {  // no pass B: one group of the next row follows each stage
-        copies_wait<kStages - 1>(), stage(0);
-        copies_wait<kStages - 1>(), stage(1);
-        copies_wait<kStages - 1>(), stage(2);
-        copies_wait<kStages - 1>(), stage(3);
-      } else {
-        copies_wait<3>(), stage(0);
-        copies_wait<2>(), stage(1);
-        copies_wait<1>(), stage(2);
-        copies_wait<0>(), stage(3);
       }
       const Stat st = combine_lanes<ENT, LABEL1>(run.get(), 32, a.c);
       if (lane == 0) part[par][wid] = st;
