@@ -129,6 +129,8 @@ class CortexError(RuntimeError):
 def load(path=None):
     """Loads libcortex.so (once) and declares every exported function."""
     global _lib
+    if _lib is not None and path is None:
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib

@@ -398,12 +398,24 @@ __device__ __forceinline__ void rebase(Stat &a, float m, float c) {
   a.m = m;
 }
 
+// exp(d) from e = exp(d / T): its square or fourth power (SQ squarings), or by itself.
+template <int SQ>
+__device__ __forceinline__ f2 at_one(f2 e, f2 d, f2 l2) {
+  if (SQ) {
+    e = mul2(e, e);
+    return SQ == 2 ? mul2(e, e) : e;
+  }
+  float a, b;
+  unpack2(mul2(d, l2), a, b);
+  return pack2(ex2(a), ex2(b));
+}
+
 // A thread's statistics as its words come.  m need not be the maximum: sums
 // relative to a value up to 2^kAbove below it are as good (a sum of 2^19 terms
 // stays far from fp32's end), so they are rebased only when a chunk's maximum
 // cm passes that: once or twice a row instead of at most chunks.
 constexpr float kAbove = 16.f;
-template <typename E, bool W, bool S1>
+template <typename E, bool W, bool S1, int SQ = 0>
 struct Running {
   float m = -FLT_MAX, most = -FLT_MAX;
   f2 s = 0, w = 0, s1 = 0;
@@ -439,10 +451,7 @@ struct Running {
         const f2 e = pack2(ex2(a), ex2(b));
         s = add2(s, e);
         if (W) w = fma2(e, x, w);
-        if (S1) {
-          unpack2(mul2(d, l2), a, b);
-          s1 = add2(s1, pack2(ex2(a), ex2(b)));
-        }
+        if (S1) s1 = add2(s1, at_one<SQ>(e, d, l2));
       }
     }
   }
@@ -1032,8 +1041,9 @@ __device__ __forceinline__ void same_ids(const int *ids, int n, int j, bool &ear
     const int4 x = v[l >> 2];
     same += (x.x == id) + (x.y == id) + (x.z == id) + (x.w == id);
   }
-  earlier = later = false;
-  if (same > 1 || j >= n)  // j >= n: the label, behind the list
+  earlier = j >= n && same > 0;  // j = n: the label, behind the list
+  later = false;
+  if (j < n && same > 1)
     for (int l = 0; l < n; ++l) earlier |= l < j && ids[l] == id, later |= l > j && ids[l] == id;
 }
 
@@ -1051,7 +1061,9 @@ __device__ __forceinline__ void cluster_meet() {
 //   alpha = (g_H ln2 W / S - G) / (S T),  beta = -g_H ln2 / (S T).
 // MODE 1: distillation, q_j the teacher's weights:
 //   grad_i = e_i alpha + gamma softmax(z)_i - what the list and the label take.
-// EXTRA: labels at T != 1, whose softmax needs exponentials of its own.  With
+// EXTRA: labels at T != 1, whose softmax needs exponentials of its own (1), or
+// at T = 2 or 4 the squares (2) or fourth powers (3) of those at hand, which
+// spares half the exponentials (distill_1024_v16384: SQFIGS).  With
 // `rest` the listed logits are taken out of the staged row (each by the thread
 // that owns its word, which finds it in a list of its own), so that the
 // unlisted mass is a sum of its own: 1 - the listed would lose a confident
@@ -1068,10 +1080,11 @@ __device__ __forceinline__ void cluster_meet() {
 // entries' weights and the loss are held in 64 bits: a handful of values a
 // row, and a loss that is a small difference of large terms.
 constexpr int kMaxEntryWarps = 2;
-template <typename E, int NT, int MODE, bool EXTRA>
+template <typename E, int NT, int MODE, int EXTRA>
 __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) snai_row_grad(const RowGradArgs a) {
   constexpr int NW = NT / 32, kN = Word<E>::kN, kWide = kChunk * NT;
   constexpr bool ENT = MODE == 0 && EXTRA, LABEL1 = MODE == 1 && EXTRA;
+  constexpr int SQ = LABEL1 ? EXTRA - 1 : 0;  // squarings that make exp(d) of exp(d / T)
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Stat part[2][NW], listed[2][kMaxEntryWarps];
   // by entry warp: the sums of q (MODE 0: g) and of q (log q - (z - top) / T), and top
@@ -1335,7 +1348,7 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
       }
       const int c0 = e0 < 0 ? -1 : e0 / (kN * kWide), c1 = e1 < 0 ? -1 : e1 / (kN * kWide);
       // pass A
-      Running<E, ENT, LABEL1> run;
+      Running<E, ENT, LABEL1, SQ> run;
 #pragma unroll 1
       for (int s = 0; s < kStages; ++s) {
         if (!a.grad && more)  // no pass B: one group of the next row follows each stage
@@ -1391,10 +1404,7 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
                 }
                 const f2 e = pack2(ex2(u), ex2(w));
                 v[k] = mul2(e, ENT ? fma2(x, be2, al2) : al2);
-                if (LABEL1) {
-                  unpack2(mul2(d, l2), u, w);
-                  v[k] = fma2(pack2(ex2(u), ex2(w)), ga2, v[k]);
-                }
+                if (LABEL1) v[k] = fma2(at_one<SQ>(e, d, l2), ga2, v[k]);
               }
               q[j] = any ? Word<E>::pack(v) : make_uint4(0u, 0u, 0u, 0u);
             }
@@ -1637,17 +1647,15 @@ int score_nt(const char *who, const ScoreArgs &a, size_t smem, int dev, cudaStre
 
 // mode 0: scores' gradient, 1: distillation; extra: as the kernel's EXTRA
 template <typename E, int NT>
-int grad_nt(const char *who, const RowGradArgs &a, int mode, bool extra, int entry, size_t smem, int dev,
+int grad_nt(const char *who, const RowGradArgs &a, int mode, int extra, int entry, size_t smem, int dev,
             cudaStream_t st) {
-  const int nt = NT + entry;
-  if (mode == 0)
-    return extra ? launch_rows(who, snai_row_grad<E, NT, 0, true>, a, nt, smem, dev, st)
-                 : launch_rows(who, snai_row_grad<E, NT, 0, false>, a, nt, smem, dev, st);
-  return extra ? launch_rows(who, snai_row_grad<E, NT, 1, true>, a, nt, smem, dev, st)
-               : launch_rows(who, snai_row_grad<E, NT, 1, false>, a, nt, smem, dev, st);
+  void (*const kern[2][4])(RowGradArgs) = {
+      {snai_row_grad<E, NT, 0, 0>, snai_row_grad<E, NT, 0, 1>, nullptr, nullptr},
+      {snai_row_grad<E, NT, 1, 0>, snai_row_grad<E, NT, 1, 1>, snai_row_grad<E, NT, 1, 2>, snai_row_grad<E, NT, 1, 3>}};
+  return launch_rows(who, kern[mode][extra], a, NT + entry, smem, dev, st);
 }
 
-int launch_row_grad(const char *who, RowGradArgs &a, int dtype, int mode, bool extra, int dev, cudaStream_t st) {
+int launch_row_grad(const char *who, RowGradArgs &a, int dtype, int mode, int extra, int dev, cudaStream_t st) {
   const int ne = a.n + (a.labels ? 1 : 0);
   const size_t lists = (size_t)((ne + 3) & ~3) * 10 * 4 + 256 * 4;
   const int entry = ne > 32 ? 64 : 32;  // entry threads
@@ -1791,7 +1799,8 @@ int launch_distill(const char *who, const DistillLaunch &s, cudaStream_t stream)
   a.loss = s.loss;
   a.grad = s.grad;
   a.grad_ld = s.grad_ld;
-  return launch_row_grad(who, a, s.dtype, 1, labels && s.temperature != 1.0, dev, stream);
+  const int extra = !labels || s.temperature == 1.0 ? 0 : s.temperature == 2.0 ? 2 : s.temperature == 4.0 ? 3 : 1;
+  return launch_row_grad(who, a, s.dtype, 1, extra, dev, stream);
 }
 
 }  // namespace snai
@@ -1860,7 +1869,7 @@ extern "C" int cortex_score_grad(const void *logits, int dtype, int rows, int vo
   a.g_entropy = g_entropy;
   a.grad = grad;
   a.grad_ld = grad_ld;
-  return launch_row_grad(who, a, dtype, 0, g_entropy != nullptr, dev, static_cast<cudaStream_t>(stream));
+  return launch_row_grad(who, a, dtype, 0, g_entropy ? 1 : 0, dev, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int cortex_distill(const void *logits, int dtype, int rows, int vocab, long long ld,

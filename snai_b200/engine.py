@@ -361,59 +361,67 @@ def sample_device(logits_dev, uniforms_dev, params, hist_dev=None, hist_len_dev=
     return out_dev
 
 
+_ROW_TYPES = {}  # torch dtype -> SNAI_DTYPE_*
+
+
+def _torch():
+    """torch, which whoever passes its tensors has imported."""
+    import torch
+
+    if not _ROW_TYPES:
+        _ROW_TYPES.update({torch.float32: _lib.DTYPE_FP32, torch.bfloat16: _lib.DTYPE_BF16,
+                           torch.float16: _lib.DTYPE_FP16})
+    return torch
+
+
 def _dev_rows(logits):
     """(dtype code, rows, vocab, row stride) of device logits [rows, vocab]."""
-    if logits.dim() != 2 or not logits.is_cuda:
-        raise CortexError("logits must be a 2-d CUDA tensor")
-    code = _DTYPES.get(str(logits.dtype))
-    if code is None:
-        raise CortexError(f"logits of type {logits.dtype}: float32, bfloat16 or float16 are taken")
+    code = _ROW_TYPES.get(logits.dtype)
+    if code is None or logits.dim() != 2 or not logits.is_cuda:
+        raise CortexError(f"logits must be a 2-d CUDA tensor of float32, bfloat16 or float16, got {logits.dtype} "
+                          f"{tuple(logits.shape)} on {logits.device}")
     rows, vocab = logits.shape
-    if vocab > 1 and logits.stride(1) != 1:
+    ld, one = logits.stride()
+    if one != 1 and vocab > 1:
         raise CortexError("the elements of a row of logits must be adjacent")
-    return code, rows, vocab, logits.stride(0) if rows > 1 else max(vocab, logits.stride(0))
-
-
-_DTYPES = {"torch.float32": _lib.DTYPE_FP32, "torch.bfloat16": _lib.DTYPE_BF16, "torch.float16": _lib.DTYPE_FP16}
+    return code, rows, vocab, ld if rows > 1 else max(vocab, ld)
 
 
 def _dev_arg(name, t, logits, shape, dtype):
     """The address of a dense device argument, None when absent."""
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape) or str(t.dtype) != dtype or t.device != logits.device or not t.is_contiguous():
+    if t.shape != shape or t.dtype != dtype or t.device != logits.device or not t.is_contiguous():
         raise CortexError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {logits.device} is needed, "
                           f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _dev_tokens(tokens, logits, rows):
+def _dev_tokens(tokens, logits, rows, dtype):
     """(address, tokens a row) of tokens [rows] or [rows, n]."""
     if tokens is None:
         return None, 0
-    if tokens.dim() not in (1, 2):
+    if tokens.dim() == 1:
+        return _dev_arg("tokens", tokens, logits, (rows,), dtype), 1
+    if tokens.dim() != 2:
         raise CortexError("tokens must be [rows] or [rows, n]")
-    n = 1 if tokens.dim() == 1 else tokens.shape[1]
-    return _dev_arg("tokens", tokens, logits, (rows,) if tokens.dim() == 1 else (rows, n), "torch.int32"), n
+    return _dev_arg("tokens", tokens, logits, (rows, tokens.shape[1]), dtype), tokens.shape[1]
 
 
-def _stream_of(stream, device):
-    """The stream's handle, and the context that new tensors are made in."""
-    import contextlib
-
-    import torch
-
+def _on(stream, device, torch, made):
+    """(stream handle, made()): the given stream's handle, or torch's current
+    stream of the device; the tensors that made() allocates belong to it."""
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream, contextlib.nullcontext()
-    return stream, torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
+        return torch._C._cuda_getCurrentRawStream(device.index), made()
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+        return stream, made()
 
 
 def _dev_grad(logits, grad, rows, vocab):
-    import torch
-
+    """(the gradient's tensor, its row stride)"""
     if grad is None:
-        grad = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
-    elif grad.shape != logits.shape or grad.dtype != logits.dtype or grad.device != logits.device or (
+        return logits.new_empty((rows, vocab)), vocab
+    if grad.shape != logits.shape or grad.dtype != logits.dtype or grad.device != logits.device or (
             vocab > 1 and grad.stride(1) != 1):
         raise CortexError("the gradient must have the logits' shape, type and device, its rows' elements adjacent")
     return grad, grad.stride(0) if rows > 1 else max(vocab, grad.stride(0))
@@ -424,21 +432,23 @@ def score_device(logits_dev, tokens_dev=None, temperature=1.0, top_k=0, want_ent
     alternatives of device logits [rows, vocab] (cortex_score), as a Score of
     device tensors.  Runs on `stream` (a handle), by default torch's current
     stream of the logits' device."""
-    import torch
-
+    torch = _torch()
     code, rows, vocab, ld = _dev_rows(logits_dev)
-    tok, n = _dev_tokens(tokens_dev, logits_dev, rows)
+    tok, n = _dev_tokens(tokens_dev, logits_dev, rows, torch.int32)
     k = int(top_k)
-    handle, made_in = _stream_of(stream, logits_dev.device)
-    dev = logits_dev.device
-    with made_in:
-        lp = None if tok is None else torch.empty(tokens_dev.shape, dtype=torch.float32, device=dev)
-        ent = torch.empty(rows, dtype=torch.float32, device=dev) if want_entropy else None
-        ids = torch.empty((rows, k), dtype=torch.int32, device=dev) if k > 0 else None
-        top = torch.empty((rows, k), dtype=torch.float32, device=dev) if k > 0 else None
-    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    check(load().cortex_score(logits_dev.data_ptr(), code, rows, vocab, ld, tok, n, float(temperature), k, at(lp),
-                              at(ent), at(ids), at(top), handle), "cortex_score")
+    new, f32 = logits_dev.new_empty, torch.float32
+
+    def made():
+        return (None if tok is None else new(tokens_dev.shape, dtype=f32),
+                new((rows,), dtype=f32) if want_entropy else None,
+                new((rows, k), dtype=torch.int32) if k > 0 else None,
+                new((rows, k), dtype=f32) if k > 0 else None)
+
+    handle, (lp, ent, ids, top) = _on(stream, logits_dev.device, torch, made)
+    rc = load().cortex_score(logits_dev.data_ptr(), code, rows, vocab, ld, tok, n, temperature, k,
+                             None if lp is None else lp.data_ptr(), None if ent is None else ent.data_ptr(),
+                             None if ids is None else ids.data_ptr(), None if top is None else top.data_ptr(), handle)
+    check(rc, "cortex_score")
     return Score(lp, ent, ids, top)
 
 
@@ -447,18 +457,18 @@ def score_grad_device(logits_dev, tokens_dev=None, g_logprob_dev=None, g_entropy
     """The gradient of sum(g_logprob * logprob) + sum(g_entropy * entropy) of
     score_device with respect to the logits (cortex_score_grad); grad_dev may
     be the logits themselves."""
+    torch = _torch()
     code, rows, vocab, ld = _dev_rows(logits_dev)
-    tok, n = _dev_tokens(tokens_dev, logits_dev, rows)
+    tok, n = _dev_tokens(tokens_dev, logits_dev, rows, torch.int32)
     if (tokens_dev is None) != (g_logprob_dev is None):
         raise CortexError("tokens and g_logprob go together")
     gl = _dev_arg("g_logprob", g_logprob_dev, logits_dev, tokens_dev.shape if tokens_dev is not None else (),
-                  "torch.float32")
-    ge = _dev_arg("g_entropy", g_entropy_dev, logits_dev, (rows,), "torch.float32")
-    handle, made_in = _stream_of(stream, logits_dev.device)
-    with made_in:
-        grad, gld = _dev_grad(logits_dev, grad_dev, rows, vocab)
-    check(load().cortex_score_grad(logits_dev.data_ptr(), code, rows, vocab, ld, tok, n, float(temperature), gl, ge,
-                                   grad.data_ptr(), gld, handle), "cortex_score_grad")
+                  torch.float32)
+    ge = _dev_arg("g_entropy", g_entropy_dev, logits_dev, (rows,), torch.float32)
+    handle, (grad, gld) = _on(stream, logits_dev.device, torch, lambda: _dev_grad(logits_dev, grad_dev, rows, vocab))
+    rc = load().cortex_score_grad(logits_dev.data_ptr(), code, rows, vocab, ld, tok, n, temperature, gl, ge,
+                                  grad.data_ptr(), gld, handle)
+    check(rc, "cortex_score_grad")
     return grad
 
 
@@ -468,26 +478,25 @@ def distill_device(logits_dev, teacher_ids_dev, teacher_logits_dev, labels=None,
     top logits [rows, k] (cortex_distill), and the gradient of
     sum(row_grad * loss), which may take the logits' place (grad_dev).
     Returns (loss [rows], gradient or None)."""
-    import torch
-
+    torch = _torch()
     code, rows, vocab, ld = _dev_rows(logits_dev)
     if teacher_ids_dev.dim() != 2:
         raise CortexError("teacher_ids must be [rows, k]")
-    k = teacher_ids_dev.shape[1]
-    ids = _dev_arg("teacher_ids", teacher_ids_dev, logits_dev, (rows, k), "torch.int32")
-    vals = _dev_arg("teacher_logits", teacher_logits_dev, logits_dev, (rows, k), "torch.float32")
-    y = _dev_arg("labels", labels, logits_dev, (rows,), "torch.int32")
-    rg = _dev_arg("row_grad", row_grad, logits_dev, (rows,), "torch.float32")
-    prm = distill_params(temperature, label_weight, rest)
-    handle, made_in = _stream_of(stream, logits_dev.device)
-    grad, gld = None, 0
-    with made_in:
-        loss = torch.empty(rows, dtype=torch.float32, device=logits_dev.device)
-        if want_grad:
-            grad, gld = _dev_grad(logits_dev, grad_dev, rows, vocab)
-    check(load().cortex_distill(logits_dev.data_ptr(), code, rows, vocab, ld, ids, vals, k, y, rg, ctypes.byref(prm),
-                                loss.data_ptr(), None if grad is None else grad.data_ptr(), gld, handle),
-          "cortex_distill")
+    k, f32 = teacher_ids_dev.shape[1], torch.float32
+    ids = _dev_arg("teacher_ids", teacher_ids_dev, logits_dev, (rows, k), torch.int32)
+    vals = _dev_arg("teacher_logits", teacher_logits_dev, logits_dev, (rows, k), f32)
+    y = _dev_arg("labels", labels, logits_dev, (rows,), torch.int32)
+    rg = _dev_arg("row_grad", row_grad, logits_dev, (rows,), f32)
+
+    def made():
+        grad, gld = _dev_grad(logits_dev, grad_dev, rows, vocab) if want_grad else (None, 0)
+        return logits_dev.new_empty((rows,), dtype=f32), grad, gld
+
+    handle, (loss, grad, gld) = _on(stream, logits_dev.device, torch, made)
+    rc = load().cortex_distill(logits_dev.data_ptr(), code, rows, vocab, ld, ids, vals, k, y, rg,
+                               ctypes.byref(distill_params(temperature, label_weight, rest)), loss.data_ptr(),
+                               None if grad is None else grad.data_ptr(), gld, handle)
+    check(rc, "cortex_distill")
     return loss, grad
 
 
