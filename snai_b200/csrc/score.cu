@@ -1030,23 +1030,6 @@ __device__ __forceinline__ double exp_d(double x) {
   return e * __hiloint2double((1023 + (int)n) << 20, 0);
 }
 
-// Which of a list's n entries name the same id as entry j: an earlier one, a
-// later one.  (The entries that fill up the last four are no ids.)
-__device__ __forceinline__ void same_ids(const int *ids, int n, int j, bool &earlier, bool &later) {
-  const int id = ids[j];
-  const int4 *v = reinterpret_cast<const int4 *>(ids);
-  int same = 0;
-#pragma unroll 4
-  for (int l = 0; l < n; l += 4) {
-    const int4 x = v[l >> 2];
-    same += (x.x == id) + (x.y == id) + (x.z == id) + (x.w == id);
-  }
-  earlier = j >= n && same > 0;  // j = n: the label, behind the list
-  later = false;
-  if (j < n && same > 1)
-    for (int l = 0; l < n; ++l) earlier |= l < j && ids[l] == id, later |= l > j && ids[l] == id;
-}
-
 // Barrier of the cluster behind one thread's writes (the caller's thread 0,
 // which has fenced them): the other threads' gradient stores need not have
 // drained, as a release by every thread would have them.
@@ -1134,7 +1117,7 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
     copies_wait<0>();
   } else {
     for (int s = 0; s < kStages; ++s) cur.load(s, cps, buf);
-    if (rest) head[t] = -1;
+    head[t] = -1;
   }
   __syncthreads();
   int par = 0;
@@ -1192,6 +1175,14 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
 
   if (entry) {
     E *before = nullptr;  // the row whose entries' gradients are pending
+    auto entry_sync = [&] {
+      if (nwe > 1)
+        asm volatile("bar.sync 1, %0;" ::"r"(nte) : "memory");
+      else
+        __syncwarp();
+    };
+    // the thread that owns an id's word, when it is in this slice; equal for equal ids
+    auto hash = [&](int id) { return (unsigned)(id - cur.base + (1 << 20)) / kN % NT; };
     auto store_pending = [&] {
       if (before)
         for (int j = et; j < ne; j += nte)
@@ -1206,20 +1197,30 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
       const float sc = ENT || (MODE == 1 && a.row_grad) ? scal[par] : 1.f;
       bool any = ENT && et == 0 && sc != 0.f;  // anything but padding in the row?
       unsigned firsts = 0, again = 0;          // by entry of this thread: the id's first; listed again later
+      // the entries' logits are asked for first (one a thread without waiting)
+      const float z0 = et < ne && valid(ids[et]) ? load_now(cur.at(ids[et])) : -INFINITY;
+      for (int j = et; j < ne; j += nte) {
+        const int id = ids[j];
+        if (!valid(id)) continue;
+        any = true;
+        link[j] = make_int2(cur.local(id), atomicExch(&head[hash(id)], j));
+      }
+      // behind the barrier owners find the listed logits among their words,
+      // and entries those that name the same id
+      if (rest)
+        __syncthreads();
+      else
+        entry_sync();
       for (int j = et, i = 0; j < ne; j += nte, ++i) {
         const int id = ids[j];
         if (!valid(id)) continue;
-        bool earlier, later;
-        same_ids(ids, n, j, earlier, later);
-        firsts |= earlier ? 0u : 1u << i;
-        again |= later ? 1u << i : 0u;
-        any = true;
-        const int e = cur.local(id);
-        if (rest && !earlier && j < n && e >= 0) link[j] = make_int2(e, atomicExch(&head[e / kN % NT], j));
+        firsts |= 1u << i;
+        for (int l = head[hash(id)]; l >= 0; l = link[l].y)
+          if (ids[l] == id && l != j) {
+            if (l < j) firsts &= ~(1u << i);
+            if (l > j && l < n) again |= 1u << i;
+          }
       }
-      if (rest) __syncthreads();  // the owners may take the links
-#pragma unroll 2
-      for (int j = et; j < ne; j += nte) zl[j] = valid(ids[j]) ? Word<E>::one(cur.at(ids[j])) : -INFINITY;
       double lse = 0;
       if (MODE == 1 && !rest) {  // the teacher's log normaliser, by every entry warp
         float tm = -INFINITY, s = 0.f;
@@ -1231,6 +1232,7 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
         s = warp_sum(s);
         lse = tm == -INFINITY ? 0.0 : tm * a.inv_t + (double)logf(s);
       }
+      for (int j = et; j < ne; j += nte) zl[j] = j == et ? z0 : valid(ids[j]) ? Word<E>::one(cur.at(ids[j])) : -INFINITY;
       // logits are taken relative to the warp's greatest, so that a row of the type's lowest values keeps its differences
       float top = 0.f;
       if (MODE == 1) {
@@ -1302,7 +1304,7 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
         }
         before = static_cast<E *>(a.grad) + (long long)r * a.grad_ld;
       }
-      if (MODE == 1 && et == 0 && rank == 0) {
+      if (MODE == 1 && et == nte - 32 && rank == 0) {
         double l = 0;
         if (a.a < 1.0) {
           if (S == 0.f) {
@@ -1317,11 +1319,9 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
         if (y >= 0) l += a.a * (label_z == -INFINITY ? INFINITY : (double)m - label_z + log((double)S1));
         a.loss[r] = !any ? 0.f : S != S ? NAN : (float)l;
       }
-      // what the entry warps share of a row (weights, sums, the label's logit) is overwritten by the next
-      if (nwe > 1)
-        asm volatile("bar.sync 1, %0;" ::"r"(nte) : "memory");
-      else
-        __syncwarp();
+      for (int j = et; j < ne; j += nte)
+        if (valid(ids[j])) head[hash(ids[j])] = -1;
+      entry_sync();  // what the entry warps share of a row is overwritten by the next
       if (r + step < a.in.rows) cur.next(a.in, r, step, rank);
     }
     __syncthreads();
@@ -1340,10 +1340,9 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
         __syncthreads();
         others = head[t];
         if (others >= 0) {
-          head[t] = -1;
-          int2 l = link[others];
+          int2 l = others < n ? link[others] : make_int2(-1, link[others].y);
           e0 = l.x, others = l.y;
-          if (others >= 0) l = link[others], e1 = l.x, others = l.y;
+          if (others >= 0) l = link[others], e1 = others < n ? l.x : -1, others = l.y;
         }
       }
       const int c0 = e0 < 0 ? -1 : e0 / (kN * kWide), c1 = e1 < 0 ? -1 : e1 / (kN * kWide);
@@ -1362,7 +1361,7 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
             if (c1 == c) Word<E>::put(reinterpret_cast<E *>(buf) + e1, -INFINITY);
             for (int j = others; j >= 0;) {
               const int2 l = link[j];
-              if (l.x / (kN * kWide) == c) Word<E>::put(reinterpret_cast<E *>(buf) + l.x, -INFINITY);
+              if (j < n && l.x >= 0 && l.x / (kN * kWide) == c) Word<E>::put(reinterpret_cast<E *>(buf) + l.x, -INFINITY);
               j = l.y;
             }
           }
