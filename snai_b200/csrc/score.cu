@@ -41,7 +41,6 @@ constexpr int kMaxList = kScoreMaxK;
 constexpr int kMaxVocab = 1 << 19;  // as cortex_sample
 constexpr int kStages = 4;          // copy groups a row's words are committed in
 constexpr int kChunk = 4;           // words a thread takes at a time
-constexpr int kMaxCap = 2048;       // candidates of alternatives held at most
 constexpr float kLowest = -200.f;   // exponents (base 2) are cut here: 2^-200 is 0 in fp32, and 0 * d stays 0
 constexpr float kLn2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
 
@@ -538,20 +537,18 @@ __device__ __forceinline__ float unordered(int k) { return __int_as_float(k ^ ((
 
 // A value that at least k <= 32 N of the warp's 32 N values reach and few
 // more do.  Few: the greatest are taken off one after the other; else
-// bisection, ended a little early.
+// bisection, ended a little early.  Values are ordered integers.
+constexpr int kNone = (int)0x80000000;  // below all of them
 template <int N>
-__device__ __forceinline__ float warp_kth(const float *v, int k) {
-  int x[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = ordered(v[i]);
+__device__ __forceinline__ int warp_kth(int *x, int k) {
   if (N == 1 && k <= 8) {
     int top, c = 0;
     do {
       top = __reduce_max_sync(0xffffffffu, x[0]);
       c += __popc(__ballot_sync(0xffffffffu, x[0] == top));
-      if (x[0] == top) x[0] = (int)0x80000000;
+      if (x[0] == top) x[0] = kNone;
     } while (c < k);
-    return unordered(max(top, (int)0x807fffff));
+    return top;
   }
   int lo = x[0], hi = x[0];
 #pragma unroll
@@ -571,128 +568,155 @@ __device__ __forceinline__ float warp_kth(const float *v, int k) {
       hi = mid - 1;
     }
   }
-  return unordered(max(lo, (int)0x807fffff));
+  return lo;
+}
+// Such a value as a float: -inf when it lies below all logits.
+__device__ __forceinline__ float as_bound(int v) { return unordered(max(v, (int)0x807fffff)); }
+
+// The upper half of a sort key as an ordered integer; an empty key is kNone.
+__device__ __forceinline__ int key_order(unsigned long long key) { return (int)(unsigned)(key >> 32) ^ kNone; }
+
+// Sorts the warp's 32 keys, descending.
+__device__ __forceinline__ unsigned long long warp_sort(unsigned long long key) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll 1
+    for (int s = size / 2; s > 0; s /= 2) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, s);
+      const bool greater = ((lane & s) == 0) == ((lane & size) == 0);
+      key = (other > key) == greater ? other : key;
+    }
+  return key;
 }
 
-// A value that at least k of n values reach and few more do (their k-th
-// largest, or a little less), by one warp; -inf when n < k.  The values are
-// ordered integers, `pitch` of them apart (1: an array of them, 2: the upper
-// halves of sort keys, whose order has its sign bit flipped).
-__device__ __noinline__ float about_kth(const int *v, int pitch, int n, int k) {
-  if (n < k) return -INFINITY;
-  const int lane = threadIdx.x & 31, flip = pitch == 2 ? (int)0x80000000 : 0;
-  int lo = 0x7fffffff, hi = (int)0x80000000;
+// The place among n keys of one of them: the number of greater keys.
+__device__ __forceinline__ int place_by_counting(const unsigned long long *cand, int n, unsigned long long key) {
+  int at = n & 1 ? cand[n - 1] > key : 0;
 #pragma unroll 4
-  for (int i = lane; i < n; i += 32) {
-    const int x = v[i * pitch] ^ flip;
-    lo = min(lo, x), hi = max(hi, x);
+  for (int j = 0; j + 1 < n; j += 2) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(cand + j);
+    at += (v.x > key) + (v.y > key);
   }
-  lo = __reduce_min_sync(0xffffffffu, lo);  // k values reach lo
-  hi = __reduce_max_sync(0xffffffffu, hi);
-  const int slack = k + (k >> 2) + 2;
-  while (lo < hi) {
-    const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) >> 1);
-    int c = 0;
-#pragma unroll 8
-    for (int i = lane; i < n; i += 32) c += (v[i * pitch] ^ flip) >= mid;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (c >= k) {
-      lo = mid;
-      if (c <= slack) break;
-    } else {
-      hi = mid - 1;
-    }
-  }
-  return unordered(max(lo, (int)0x807fffff));  // -inf: below it lie no logits, only the empty keys of a buffer
+  return at;
 }
-__device__ __forceinline__ const int *upper_halves(const unsigned long long *keys) {
-  return reinterpret_cast<const int *>(keys) + 1;
+// The same among sorted runs of 32, by bisection in each.
+__device__ __noinline__ int place_in_runs(const unsigned long long *cand, int n, unsigned long long key) {
+  int at = 0;
+#pragma unroll 2
+  for (int r = 0; r < n; r += 32) {
+    const unsigned long long *run = cand + r;
+    int p = 0;
+#pragma unroll
+    for (int h = 16; h > 0; h /= 2)
+      if (run[p + h - 1] > key) p += h;
+    at += p + (run[p] > key);
+  }
+  return at;
 }
 
-// Bitonic sort of n keys, descending; room for the next power of two.  The
-// whole block calls it.
-template <int NT>
-__device__ __noinline__ void sort_keys(unsigned long long *key, int n) {
-  int len = 512;
-  while (len < n) len *= 2;
-  for (int i = n + (int)threadIdx.x; i < len; i += NT) key[i] = 0;
-  for (int size = 2; size <= len; size *= 2)
-    for (int stride = size / 2; stride > 0; stride /= 2) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < len / 2; i += NT) {
-        const int x = 2 * i - (i & (stride - 1)), y = x + stride;
-        const unsigned long long u = key[x], v = key[y];
-        if ((u < v) == ((x & size) == 0)) key[x] = v, key[y] = u;
-      }
-    }
-  __syncthreads();
-}
-
-// Writes the k greatest of n keys (k <= n; ids and log p, in order): by
-// counting the greater ones when they are few, else by a sort.  The whole
-// block calls it.
+// Writes the k greatest of n keys (k <= n; ids and log p, in order).  A key's
+// place is found by counting the greater ones when the keys are few (n^2 / 2
+// wide loads), else in sorted runs of 32 (n^2 / 5 loads, and the sorts).  The
+// whole block calls it; room for a multiple of 32.
 template <int NT>
 __device__ __forceinline__ void put_greatest(unsigned long long *cand, int n, int k, int *ids, float *lps, float m,
                                              float inv_t, float s) {
   const int t = threadIdx.x;
-  const bool sorted = n > 384;
-  if (sorted) sort_keys<NT>(cand, n);
+  const bool runs = n > 96;
+  if (runs) {
+    for (int i = t; i < (n + 31) / 32 * 32; i += NT) cand[i] = warp_sort(i < n ? cand[i] : 0);
+    __syncthreads();
+  }
   const float ls = logf(s);
-  for (int i = t; i < (sorted ? k : n); i += NT) {
+  for (int i = t; i < n; i += NT) {
     const unsigned long long key = cand[i];
-    int at = i;
-    if (!sorted) {
-      at = n & 1 ? cand[n - 1] > key : 0;
-#pragma unroll 4
-      for (int j = 0; j + 1 < n; j += 2) {
-        const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(cand + j);
-        at += (v.x > key) + (v.y > key);
-      }
-    }
-    if (at < k) {
+    const int at = runs ? place_in_runs(cand, n, key) : place_by_counting(cand, n, key);
+    if (at < k && key) {
       ids[at] = key_id(key);
       lps[at] = log_p(key_logit(key), m, inv_t, s, ls);
     }
   }
 }
 
+// Candidates held at most.  128 threads take rows with up to kFewTop
+// alternatives, 256 those with more.
+constexpr int kFewTop = 32;
+constexpr int max_cap(int nt) { return nt == 128 ? 512 : 2048; }
+
 // What the block's threads share of a row's candidates.
 struct Pool {
   unsigned long long *key;  // cap of them
   int *n;                   // collected (may pass cap)
   int *ge;
-  float *tau;
+  int *bound;  // one a warp
   int cap;
 };
 
-// Thins out a pool of n <= cap candidates: about the k greatest stay; returns
-// the value they reach.  The whole block calls it, after a barrier.
-template <int NT>
+// Thins out a pool of n <= N NT candidates: those stay that reach the least of
+// the values which each warp's share of k of its part of them reaches, at
+// least k in all.  Returns that value.  The whole block calls it, after a
+// barrier.
+template <int NT, int N>
 __device__ __noinline__ float thin_out(const Pool p, int n, int k) {
-  const int t = threadIdx.x;
-  if (t < 32) {
-    const float b = about_kth(upper_halves(p.key), 2, n, k);
-    if (t == 0) *p.tau = b, *p.n = 0;
+  constexpr int NW = NT / 32;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  unsigned long long own[N];
+  int x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int j = i * NT + lane * NW + wid;  // spread evenly over the warps
+    own[i] = j < n ? p.key[j] : 0;
+    x[i] = key_order(own[i]);
+  }
+  const int b = warp_kth<N>(x, (k + NW - 1) / NW);
+  if (lane == 0) p.bound[wid] = b;
+  __syncthreads();
+  const int tau = __reduce_min_sync(0xffffffffu, p.bound[lane % NW]);
+  if (threadIdx.x == 0) *p.n = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const bool keep = own[i] && key_order(own[i]) >= tau;
+    const unsigned all = __ballot_sync(0xffffffffu, keep);
+    if (!all) continue;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(p.n, __popc(all));
+    at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << lane) - 1));
+    if (keep) p.key[at] = own[i];
   }
   __syncthreads();
-  const float tau = *p.tau;
-  unsigned long long own[kMaxCap / NT];
-  int m = 0;
-#pragma unroll
-  for (int i = 0; i < kMaxCap / NT; ++i) {
-    own[i] = i * NT + t < n ? p.key[i * NT + t] : 0;
-    if (key_logit(own[i]) >= tau)  // an empty key is no number
-      ++m;
-    else
-      own[i] = 0;
+  return as_bound(tau);
+}
+
+// A value that at least k of n keys reach and few more do, by one warp; -inf when n < k.
+__device__ __noinline__ float about_kth(const unsigned long long *key, int n, int k) {
+  if (n < k) return -INFINITY;
+  const int lane = threadIdx.x & 31;
+  int lo = 0x7fffffff, hi = kNone;
+  for (int i = lane; i < n; i += 32) lo = min(lo, key_order(key[i])), hi = max(hi, key_order(key[i]));
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  while (lo < hi) {
+    const int mid = lo + (int)(((unsigned)hi - (unsigned)lo + 1u) >> 1);
+    int c = 0;
+    for (int i = lane; i < n; i += 32) c += key_order(key[i]) >= mid;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= k) {
+      lo = mid;
+      if (c <= k + (k >> 2) + 2) break;
+    } else {
+      hi = mid - 1;
+    }
   }
-  __syncthreads();
-  int at = m ? atomicAdd(p.n, m) : 0;
-#pragma unroll
-  for (int i = 0; i < kMaxCap / NT; ++i)
-    if (own[i]) p.key[at++] = own[i];
-  __syncthreads();
-  return tau;
+  return as_bound(lo);
+}
+
+template <int NT>
+__device__ __forceinline__ float thin_out(const Pool p, int n, int k) {
+  if (n <= NT) return thin_out<NT, 1>(p, n, k);
+  if (NT == 128 || n <= 4 * NT) return thin_out<NT, 4>(p, n, k);
+  return thin_out<NT, max_cap(NT) / NT>(p, n, k);
 }
 
 // f(z, id) for this thread's logits >= least of `words` words a thread, the
@@ -773,14 +797,13 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Stat part[2][NW];
   __shared__ Slip slip[2];
-  __shared__ float bound[2][NW], tau_s;
-  __shared__ int n_cand[2], n_ge, n_lead;
+  __shared__ int bound[2][NW], n_cand[2], n_ge, n_lead;
   uint4 *ring = reinterpret_cast<uint4 *>(smem);
   // candidates, then (rank 0 of a cluster) those of all slices
   unsigned long long *cand = reinterpret_cast<unsigned long long *>(smem + D * kWide * 16);
   unsigned long long *gath = cand + a.cap;
   int par = 0;
-  auto pool = [&] { return Pool{cand, &n_cand[par], &n_ge, &tau_s, a.cap}; };
+  auto pool = [&] { return Pool{cand, &n_cand[par], &n_ge, bound[par], a.cap}; };
   const int t = threadIdx.x, lane = t & 31, wid = t >> 5;
   const int C = a.in.C;
   const unsigned rank = C > 1 ? cluster_ctarank() : 0;
@@ -845,19 +868,21 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
           // groups of four words, two, or one; all reach the least of these.
           constexpr int kFew = 8;
           const int k = (a.top_k + NW - 1) / NW;
-          float b;
+          int b;
           if (k <= kFew) {
-            b = warp_kth<1>(&cm, k);
+            int v = ordered(cm);
+            b = warp_kth<1>(&v, k);
           } else if (k <= 2 * kFew) {
-            const float v[2] = {max_nan(wm[0], wm[1]), max_nan(wm[2], wm[3])};
+            int v[2] = {ordered(max_nan(wm[0], wm[1])), ordered(max_nan(wm[2], wm[3]))};
             b = warp_kth<2>(v, k);
           } else {
-            b = warp_kth<4>(wm, k);
+            int v[4] = {ordered(wm[0]), ordered(wm[1]), ordered(wm[2]), ordered(wm[3])};
+            b = warp_kth<4>(v, k);
           }
           if (lane == 0) bound[par][wid] = b;
           if (t == 0) n_cand[par] = 0;
           __syncthreads();
-          tau = least = -warp_max_nan(-bound[par][lane % NW]);
+          tau = least = as_bound(__reduce_min_sync(0xffffffffu, bound[par][lane % NW]));
         }
         if (cm >= least) {
           // this thread's hits as bits, room for them, then their keys
@@ -900,7 +925,7 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
       else
         cut_out<E, NT>(pool(), cur, 0, chunks * kChunk, tau, a.top_k, a.soft, [cur](int w) { return cur.fetch(w); });
       n = n_cand[par];
-    } else if (TOPK && n > 96 && n > 3 * a.top_k) {  // cheaper than ordering them all
+    } else if (TOPK && n > 128 && n > 3 * a.top_k) {  // cheaper than ordering them all
       thin_out<NT>(pool(), n, a.top_k);
       n = n_cand[par];
     }
@@ -910,7 +935,7 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
         st = combine_lanes<ENT, false>(part[par][lane % NW], NW, a.c);
         if (TOPK)
           tau = st.s != st.s ? INFINITY
-                             : about_kth(upper_halves(cand), 2, n, (a.top_k + C - 1) / C);
+                             : about_kth(cand, n, (a.top_k + C - 1) / C);
         if (lane == 0) slip[par].st = st, slip[par].tau = tau, n_lead = 0;
       }
       cluster_sync_all();
@@ -1554,7 +1579,7 @@ Plan plan_stream(const void *logits, int dtype, int rows, int vocab, long long l
   p.C = 1;
   while (p.C < 8 && (long long)rows * p.C * 2 <= 2 * sms && words / (2 * p.C) >= 512) p.C *= 2;
   p.wps = (words + p.C - 1) / p.C;
-  p.nt = p.wps <= 1024 || top_k <= 32 ? 128 : 256;
+  p.nt = top_k <= kFewTop ? 128 : 256;
   p.even = ld * elem_size(dtype) % 16 == 0;
   return p;
 }
@@ -1726,7 +1751,7 @@ int launch_score(const char *who, const ScoreLaunch &s, cudaStream_t stream) {
   // times as many of the next three: with room for 10 k the block meets each
   // time the row has grown fourfold, else each time it has doubled.
   a.soft = s.top_k + s.top_k / 2 + 16;
-  for (a.cap = 512; a.cap < kMaxCap && a.cap < 10 * s.top_k;) a.cap *= 2;
+  for (a.cap = 512; a.cap < max_cap(s.top_k <= kFewTop ? 128 : 256) && a.cap < 10 * s.top_k;) a.cap *= 2;
   a.grow = a.cap >= 10 * s.top_k ? 4 : 2;
   const Plan p = plan_stream(s.logits, s.dtype, s.rows, s.V, s.ld, s.top_k, device_sm_count(dev));
   a.in.wps = p.wps;
