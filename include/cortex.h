@@ -378,10 +378,11 @@ CORTEX_API int cortex_train_info(void *state, int *adam_steps, float *clip_facto
 /* vocabulary logits in device memory (beside cortex_sample), then the same  */
 /* on a state's own passes and training step.                                */
 /*                                                                           */
-/* logits[rows][ld] (row stride ld >= vocab, vocab <= 524288) are fp32, bf16 */
-/* or fp16; any alignment of the rows to an element is taken, 16-byte        */
-/* aligned rows are fastest.  p = softmax(logits / temperature) of a row,    */
-/* 0.001 <= temperature <= 1000.  Statistics are held in fp32 or more.       */
+/* logits[rows][ld] (row stride ld >= vocab, vocab <= 524288, rows <= 2^30,  */
+/* rows * ld <= 2^48) are fp32, bf16 or fp16; any alignment of the rows to   */
+/* an element is taken, 16-byte aligned rows are fastest.  Within a row,     */
+/* p = softmax(logits / temperature), 0.001 <= temperature <= 1000.          */
+/* Statistics are held in fp32 or more.                                      */
 /*  - An id outside [0, vocab) is padding: log probability 0, no teacher     */
 /*    mass, no gradient.                                                     */
 /*  - A logit of -inf is masked: p = 0, log p = -inf, gradient 0.  A row     */
@@ -391,8 +392,9 @@ CORTEX_API int cortex_train_info(void *state, int *adam_steps, float *clip_facto
 /* Work is queued on `stream` (a cudaStream_t of the device that holds the   */
 /* arrays; NULL = its legacy default stream), whichever device is current;   */
 /* nothing is allocated and no workspace is shared, so calls may overlap and */
-/* be captured into CUDA graphs.  Results do not depend on the other rows of */
-/* a call, and repeat bit for bit.                                           */
+/* be captured into CUDA graphs.  A call repeats bit for bit.  What a row     */
+/* holds does not reach another's results; how many rows a call has may       */
+/* change how each is spread over the GPU, and so the order of its sums.      */
 /* ------------------------------------------------------------------------ */
 
 #define SNAI_DTYPE_FP32 0

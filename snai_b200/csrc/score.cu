@@ -11,13 +11,20 @@
 // (its alternatives' ids -1).
 //
 // All three read a row once from memory and are bound by that (and by the
-// gradient's one write).  A row lives in shared memory, cut into slices over
-// a cluster of CTAs when it is long: 16-byte words copied asynchronously,
-// each by the thread that will read it, so no barrier stands between a copy
-// and its use, and the next row's copies go out as soon as a thread is done
-// with its words.  Pass A gathers m, S and sum(e d) together (a running
-// maximum per thread, checked once per chunk of four words); what comes
-// after it - alternatives, gradient - reads shared memory only.
+// gradient's one write).  16-byte words are copied to shared memory
+// asynchronously, each by the thread that will read it, so no barrier stands
+// between a copy and its use.  Pass A takes four words at a time (a chunk) and
+// gathers the reference m, S and sum(e d) together.  Scores need no more and
+// stream through a ring; a gradient needs the row again, which stays staged,
+// cut into slices over a cluster of CTAs when it is long.
+//
+// Measured on a B200 against its copy rate of 6553 GB/s (the bytes each
+// operator cannot do without over its time): 8192 x 16384 fp32 scores 0.91,
+// with 20 alternatives 0.60, gradient 0.87, distillation of 64 entries with
+// labels 0.78; 8192 x 32000 bf16 scores 0.82, 2048 x 131072 bf16 gradient 0.78
+// (issue-bound: 11 lane instructions for two bytes of an element; an eighth or
+// a quarter of the exponentials on the FMA pipe made it slower); 2048 x 131072
+// fp32 scores 0.95, with 64 alternatives 0.73, distillation with the rest 0.75.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -39,6 +46,8 @@ namespace {
 
 constexpr int kMaxList = kScoreMaxK;
 constexpr int kMaxVocab = 1 << 19;  // as cortex_sample
+constexpr int kMaxRows = 1 << 30;
+constexpr long long kMaxElems = 1ll << 48;  // rows x stride: byte offsets stay far inside 64 bits
 constexpr int kStages = 4;          // copy groups a row's words are committed in
 constexpr int kChunk = 4;           // words a thread takes at a time
 constexpr float kLowest = -200.f;   // exponents (base 2) are cut here: 2^-200 is 0 in fp32, and 0 * d stays 0
@@ -747,10 +756,10 @@ __device__ __noinline__ float cut_out(const Pool p, const Slice<E, NT> s, int w0
                                       Get word) {
   const int t = threadIdx.x;
   unsigned long long lo = sort_key(tau, INT_MAX), hi = ~0ull;
-  for (;;) {
-    const unsigned long long mid = lo + ((hi - lo) >> 1) + 1;
+  while (lo < hi) {  // a row with NaNs may have fewer than k numbers: it ends all the same
+    const unsigned long long mid = lo + ((hi - lo - 1) >> 1) + 1;
     __syncthreads();
-    if (t == 0) *p.ge = *p.n = 0;
+    if (t == 0) *p.ge = 0;
     __syncthreads();
     int g = 0;
     each_logit(s, w0, words, key_logit(mid), word, [&](float z, int id) { g += sort_key(z, id) >= mid; });
@@ -765,6 +774,8 @@ __device__ __noinline__ float cut_out(const Pool p, const Slice<E, NT> s, int w0
       if (g <= few) break;
     }
   }
+  if (t == 0) *p.n = 0;
+  __syncthreads();
   each_logit(s, w0, words, key_logit(lo), word, [&](float z, int id) {
     if (sort_key(z, id) >= lo) p.key[atomicAdd(p.n, 1)] = sort_key(z, id);
   });
@@ -890,7 +901,7 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
           const unsigned lim = Word<E>::limit(least);
 #pragma unroll
           for (int j = 0; j < kChunk; ++j)
-            if (wm[j] >= least) hits |= Word<E>::reach(q[j], lim) << (j * kN);
+            if (wm[j] >= least && c * kWide + j * NT + t < cur.n) hits |= Word<E>::reach(q[j], lim) << (j * kN);
           for (int p = atomicAdd(&n_cand[par], __popc(hits)); hits; hits &= hits - 1, ++p) {
             const int b = __ffs(hits) - 1, j = b / kN, k = b % kN, id = cur.id0(c * kWide + j * NT + t) + k;
             const float z = Word<E>::one(reinterpret_cast<const E *>(at + j * NT + t) + k);
@@ -907,7 +918,7 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
                          : cut_out<E, NT>(pool(), cur, 0, (c + 1) * kChunk, tau, a.top_k, a.soft,
                                           [cur](int w) { return cur.fetch(w); });
           else if (n > a.soft)
-            tau = thin_out<NT>(pool(), n, a.top_k);
+            tau = fmaxf(tau, thin_out<NT>(pool(), n, a.top_k));
           if (c == meet) meet = a.grow * (meet + 1) - 1;
         }
         least = next_up(tau);
@@ -981,8 +992,8 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
         cluster_sync_all();
         int m = (int)ld_cluster_u32(to_n);
         if (m > a.cap) {  // ties over several slices: bisect
-          for (;;) {
-            const unsigned long long mid = lo + ((hi - lo) >> 1) + 1;
+          while (lo < hi) {
+            const unsigned long long mid = lo + ((hi - lo - 1) >> 1) + 1;
             cluster_sync_all();
             if (t == 0) n_ge = 0, n_lead = 0;
             cluster_sync_all();
@@ -1070,24 +1081,27 @@ __device__ __forceinline__ void cluster_meet() {
 // MODE 1: distillation, q_j the teacher's weights:
 //   grad_i = e_i alpha + gamma softmax(z)_i - what the list and the label take.
 // EXTRA: labels at T != 1, whose softmax needs exponentials of its own (1), or
-// at T = 2 or 4 the squares (2) or fourth powers (3) of those at hand, which
-// spares half the exponentials (distill_1024_v16384: SQFIGS).  With
-// `rest` the listed logits are taken out of the staged row (each by the thread
-// that owns its word, which finds it in a list of its own), so that the
-// unlisted mass is a sum of its own: 1 - the listed would lose a confident
-// student's.
+// at T = 2 or 4 the squares (2) or fourth powers (3) of those at hand
+// (16384 x 8192, 64 entries: 211 us against 225 with exponentials of their
+// own; 4096 x 32000 bf16: 135 against 169).  With `rest` the listed logits
+// are taken out of the staged row (each by the thread that owns its word,
+// which finds it in a list of its own), so that the unlisted mass is a sum of
+// its own: 1 - the listed would lose a confident student's.
 //
 // The first NT threads stage the row and take it through both passes; 32 or
-// 64 more, the entry threads, have the list: they work a row ahead, with the
+// 64 more, the entry threads, have the list: they work beside pass A, with the
 // entries' logits read from global memory, so that what a row costs the others
 // is one barrier (`rest`: two) and the scalars, which every warp then works
 // out.  Pass B writes the terms that every element has; the entries' ids get
 // theirs from the entry threads one row later, behind the next row's barrier,
-// when all owners have written the base.  An id listed more than once is
-// handled by its first entry, in the order of the list: no atomics.  The
-// entries' weights and the loss are held in 64 bits: a handful of values a
-// row, and a loss that is a small difference of large terms.
-constexpr int kMaxEntryWarps = 2;
+// when all owners have written the base.  (Entries held by threads that also
+// take the row took 46 us where this takes 34, at 1024 x 16384 with 64 entries
+// and labels: their chain of dependent steps is as long as both passes.)  An
+// id listed more than once is handled by its first entry, in the order of the
+// list: no atomics.  The entries' weights and the loss are held in 64 bits: a
+// handful of values a row, and a loss that is a small difference of large
+// terms.
+constexpr int kMaxEntryWarps = 2;  // more would cost the third CTA of an SM its registers
 template <typename E, int NT, int MODE, int EXTRA>
 __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) snai_row_grad(const RowGradArgs a) {
   constexpr int NW = NT / 32, kN = Word<E>::kN, kWide = kChunk * NT;
@@ -1504,16 +1518,16 @@ int check_rows(const char *who, const void *logits, int dtype, int rows, int voc
     set_error("%s: unknown dtype %d", who, dtype);
     return -2;
   }
-  if (rows < 0) {
-    set_error("%s: rows < 0", who);
+  if (rows < 0 || rows > kMaxRows) {
+    set_error("%s: rows %d outside [0, %d]", who, rows, kMaxRows);
     return -2;
   }
   if (vocab < 1 || vocab > kMaxVocab) {
     set_error("%s: vocab %d outside [1, %d]", who, vocab, kMaxVocab);
     return -2;
   }
-  if (ld < vocab || ld > (1ll << 40)) {
-    set_error("%s: row stride %lld < vocab %d", who, ld, vocab);
+  if (ld < vocab || ld > kMaxElems / std::max(rows, 1)) {
+    set_error("%s: row stride %lld < vocab %d, or %d such rows beyond any memory", who, ld, vocab, rows);
     return -2;
   }
   if (!(t >= 1e-3 && t <= 1e3)) {
@@ -1536,8 +1550,8 @@ int check_rows(const char *who, const void *logits, int dtype, int rows, int voc
 // the same stride).
 int check_grad(const char *who, const void *logits, int dtype, int rows, int vocab, long long ld, const void *grad,
                long long gld) {
-  if (gld < vocab || gld > (1ll << 40)) {
-    set_error("%s: gradient row stride %lld < vocab %d", who, gld, vocab);
+  if (gld < vocab || gld > kMaxElems / std::max(rows, 1)) {
+    set_error("%s: gradient row stride %lld < vocab %d, or %d such rows beyond any memory", who, gld, vocab, rows);
     return -2;
   }
   const long long es = elem_size(dtype);

@@ -83,7 +83,9 @@ def distill(lib, logits=P, dtype=0, rows=2, vocab=100, ld=100, ids=P, vals=P, k=
 
 COMMON = [dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(vocab=0), dict(vocab=(1 << 19) + 1, ld=1 << 20),
           dict(ld=99), dict(ld=-100), dict(T=0.0), dict(T=-1.0), dict(T=float("nan")), dict(T=float("inf")),
-          dict(T=1e-4), dict(logits=None), dict(logits=ctypes.c_void_p((1 << 20) + 2))]
+          dict(T=1e-4), dict(logits=None), dict(logits=ctypes.c_void_p((1 << 20) + 2)),
+          dict(rows=(1 << 30) + 1), dict(rows=2 ** 31 - 1),  # rows past 2^30
+          dict(rows=1 << 30, ld=1 << 20), dict(ld=(1 << 47) + 1), dict(rows=1, ld=2 ** 63 - 1)]  # offsets past any memory
 
 
 @pytest.mark.parametrize("bad", COMMON + [
@@ -100,6 +102,7 @@ def test_score_refuses(built, bad):
     dict(n_tok=0, gh=None), dict(grad=ctypes.c_void_p((1 << 24) + 2)),
     dict(grad=ctypes.c_void_p((1 << 20) + 4)),              # one element on: overlaps
     dict(grad=ctypes.c_void_p((1 << 20) + 400)),            # one row on
+    dict(gld=1 << 60),
     dict(grad=P, gld=101)], ids=str)                        # same memory, other stride
 def test_score_grad_refuses(built, bad):
     from snai_b200 import last_error, load
