@@ -433,8 +433,9 @@ CORTEX_API int cortex_score_grad(const void *logits, int dtype, int rows, int vo
  *   and what the list leaves of 1 (at least 0) is one more outcome, set
  *   against the student's probability of all unlisted ids.  Where the student
  *   has none (every unlisted id masked) that outcome is left out.
- * A row whose list and label are all padding has loss 0 and gradient 0,
- * whatever its logits hold. */
+ * A listed q of 0 (below e^-700) adds nothing; any other against a masked
+ * logit makes the loss infinite.  A row whose list and label are all padding
+ * has loss 0 and gradient 0, whatever its logits hold. */
 typedef struct snai_distill_params {
   double temperature;
   double label_weight; /* 0 <= label_weight <= 1; above 0 needs labels */

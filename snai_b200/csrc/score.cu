@@ -1290,7 +1290,7 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
           if (valid(id)) q = vals[j];
         } else if (valid(id) && vals[j] != -INFINITY) {
           const double lq = rest ? (double)vals[j] : vals[j] * a.inv_t - lse;
-          q = rest ? exp_d(lq) : (double)expf((float)lq);
+          q = exp_d(lq);  // not fp32's: an entry of 1e-60 against a masked logit is an infinite loss all the same
           if (q != 0.0) kl_own += q * (lq - ((double)z - top) * a.inv_t);
         }
         q_own += q;

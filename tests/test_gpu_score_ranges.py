@@ -1,6 +1,8 @@
 """The vocabulary-row operators over ranges: drawn shapes, types, alignments,
 masks and lists against 64 bits, calls of very many short rows, long lists on
 short rows, what padding entries may hold, and what lies around the outputs."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -149,8 +151,8 @@ def test_lists_of_one_id(built, V):
 @pytest.mark.parametrize("R,V,dtype", [(3, 7, "bf16"), (40, 1003, "fp32"), (500, 2049, "fp16"), (9, 70001, "bf16")])
 def test_outputs_end_where_they_end(built, R, V, dtype):
     """Guards before and behind every output, the gradient in rows of its own stride."""
-    from snai_b200 import DistillParams, check, load
-    import ctypes
+    from snai_b200 import DistillParams, load
+
     rng = np.random.default_rng(R + V)
     k, n, gld = 5, 3, V + 6
     z = rows_of(rng, R, V, dtype, "mixed")
@@ -165,12 +167,12 @@ def test_outputs_end_where_they_end(built, R, V, dtype):
     p = {x: b.data_ptr() + 32 * b.element_size() for x, b in f.items()}
     lib, st, code = load(), torch.cuda.current_stream().cuda_stream, {"fp32": 0, "bf16": 1, "fp16": 2}[dtype]
     prm = DistillParams(1.0, 0.0, 0)
-    check(lib.cortex_score(t.data_ptr(), code, R, V, V + 2, tt.data_ptr(), n, 1.0, k, p["lp"], p["ent"], p["ids"],
-                           p["top"], st), "score")
-    check(lib.cortex_score_grad(t.data_ptr(), code, R, V, V + 2, tt.data_ptr(), n, 1.0, gt.data_ptr(), None, p["g1"],
-                                gld, st), "grad")
-    check(lib.cortex_distill(t.data_ptr(), code, R, V, V + 2, it.data_ptr(), vt.data_ptr(), k, None, None,
-                             ctypes.byref(prm), p["loss"], p["g2"], gld, st), "distill")
+    assert lib.cortex_score(t.data_ptr(), code, R, V, V + 2, tt.data_ptr(), n, 1.0, k, p["lp"], p["ent"], p["ids"],
+                            p["top"], st) == 0
+    assert lib.cortex_score_grad(t.data_ptr(), code, R, V, V + 2, tt.data_ptr(), n, 1.0, gt.data_ptr(), None, p["g1"],
+                                 gld, st) == 0
+    assert lib.cortex_distill(t.data_ptr(), code, R, V, V + 2, it.data_ptr(), vt.data_ptr(), k, None, None,
+                              ctypes.byref(prm), p["loss"], p["g2"], gld, st) == 0
     torch.cuda.synchronize()
     for x, b in f.items():
         assert (b[:32] == 77).all() and (b[-32:] == 77).all(), x
@@ -275,9 +277,9 @@ def test_a_run_of_them(built):
         tol = (rel_err_bound(zs[r], 1.0) + rel_err_bound(zt[r], 1.0)) * (2 * T * T + w[3]) * 2
         assert abs(got[r] - w[0]) <= tol
     want = [distill_row(zs[r], s.top_ids[r].cpu().numpy(), vals[r], int(y[r]), T, 0.5, True) for r in range(R)]
-    # q's relative error is its log's absolute one: as large as the student's own
-    check_grad(grad, np.stack([w[1] for w in want]), np.stack([w[2] for w in want]), np.concatenate([zs, zt], 1), 1.0,
-               "fp32", 2.0)
+    # q's relative error is its log's absolute one, the teacher's bound: at most twice the student's own
+    assert all(rel_err_bound(zt[r], T) <= 2 * rel_err_bound(zs[r], 1.0) for r in range(R))
+    check_grad(grad, np.stack([w[1] for w in want]), np.stack([w[2] for w in want]), zs, 1.0, "fp32", 3.0)
 
 
 @pytest.mark.parametrize("V,k,dtype", [(4, 4, "fp16"), (700, 512, "bf16"), (20000, 20, "fp32"), (70000, 512, "bf16"),
