@@ -8,6 +8,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdint>
+#include <climits>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -959,6 +960,10 @@ extern "C" int cortex_score_batch(void *state, const int *tokens, int batch, int
     set_error("tokens is NULL");
     return -2;
   }
+  if ((long long)batch * n_tok > INT_MAX) {  // a pass's rows name their tokens by int
+    set_error("cortex_score_batch: %d x %d tokens are more than %d", batch, n_tok, INT_MAX);
+    return -2;
+  }
   if (!slots_ok(e, slots, batch)) return -2;
   const bool dev = flags & SNAI_DEVICE_PTRS;
   DeviceGuard g(e.device);
@@ -967,8 +972,8 @@ extern "C" int cortex_score_batch(void *state, const int *tokens, int batch, int
   const int R = score_rows_max(e);
   std::vector<RowDesc> rows;
   std::vector<size_t> at;  // the outputs' index of each row
-  rows.reserve((size_t)batch * n_tok);
-  at.reserve((size_t)batch * n_tok);
+  rows.reserve((size_t)batch * std::min(n_tok, e.d.ctx));
+  at.reserve((size_t)batch * std::min(n_tok, e.d.ctx));
   std::vector<int> done(batch, 0);
   for (int b = 0; b < batch; ++b) {
     const int sl = slots ? slots[b] : b;

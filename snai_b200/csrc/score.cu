@@ -31,6 +31,7 @@
 #include <cfloat>
 #include <climits>
 #include <cmath>
+#include <exception>
 #include <initializer_list>
 #include <map>
 #include <mutex>
@@ -902,7 +903,7 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
 #pragma unroll
           for (int j = 0; j < kChunk; ++j)
             if (wm[j] >= least && c * kWide + j * NT + t < cur.n) hits |= Word<E>::reach(q[j], lim) << (j * kN);
-          for (int p = atomicAdd(&n_cand[par], __popc(hits)); hits; hits &= hits - 1, ++p) {
+          for (int p = hits ? atomicAdd(&n_cand[par], __popc(hits)) : 0; hits; hits &= hits - 1, ++p) {
             const int b = __ffs(hits) - 1, j = b / kN, k = b % kN, id = cur.id0(c * kWide + j * NT + t) + k;
             const float z = Word<E>::one(reinterpret_cast<const E *>(at + j * NT + t) + k);
             // the masked filling behind the row's ends is no logit: an empty key
@@ -1638,7 +1639,7 @@ int launch_rows(const char *who, void (*kern)(A), const A &args, int nt, size_t 
   static std::mutex mu;
   static std::map<std::tuple<const void *, int, int, int, size_t>, int> fits;
   int fit = 0;
-  {
+  try {
     std::lock_guard<std::mutex> g(mu);
     int &f = fits[std::make_tuple(fn, dev, C, nt, smem)];
     if (f == 0) {
@@ -1658,6 +1659,9 @@ int launch_rows(const char *who, void (*kern)(A), const A &args, int nt, size_t 
       }
     }
     fit = f;
+  } catch (const std::exception &x) {  // no exception leaves a C entry
+    set_error("%s: %s", who, x.what());
+    return -3;
   }
   cfg.gridDim = dim3((unsigned)(std::min(args.in.rows, fit) * C));
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args);

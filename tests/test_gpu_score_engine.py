@@ -138,6 +138,29 @@ def test_score_batch_refuses_before_feeding(model_dir, built):
     eng.close()
 
 
+def test_score_batch_lengths_beyond_the_context(model_dir, built):
+    """Token counts far past ctx: the positions that fit are scored; counts that no array could hold are refused."""
+    p = make_model(model_dir, "score_a.snai", 1000, 128, 96, 2, seed=5, std=0.06)
+    ref, eng = (Cortex(p, num_heads=2, max_seqs=2) for _ in range(2))
+    ctx = 96
+    t = (np.arange(ctx, dtype=np.int32) * 7 % 1000).reshape(1, ctx)
+    want = ref.score(t, t)
+    lp, ent = np.zeros(ctx, np.float32), np.zeros(ctx, np.float32)
+    args = (t.ctypes.data, t.ctypes.data, lp.ctypes.data, ent.ctypes.data)
+
+    def call(batch, n):
+        return eng.lib.cortex_score_batch(eng.h, args[0], batch, n, None, args[1], 1.0, 0, args[2], args[3], None,
+                                          None, 0)
+    assert call(2, 2 ** 31 - 1) < 0 and eng.pos(0) == 0
+    # of 2^31 - 1 tokens only the first ctx are read; the scores of a slot at its end are left alone
+    assert call(1, 2 ** 31 - 1) == 0 and eng.pos(0) == ctx
+    assert np.array_equal(lp, want.logprob[0]) and np.array_equal(ent, want.entropy[0])
+    lp[:] = 7.0
+    assert call(1, 5) == 0 and (lp == 7.0).all()
+    eng.close()
+    ref.close()
+
+
 GRAD_TOL = {PREC_FP32: 2e-5, PREC_TF32: 1e-2}
 KEYS = [(-1, 0), (-1, 1), (-1, 2)] + [(l, t) for l in range(2) for t in (10, 11, 12, 13, 14, 15, 16, 17)]
 
