@@ -1587,12 +1587,18 @@ int row_words(const void *logits, int dtype, int vocab, long long ld) {
 
 // Streamed rows: a CTA a row, whatever its length.  When the rows leave SMs
 // short of CTAs a row is spread over a cluster of up to 8, down to slices of
-// 8 KB.
+// 8 KB: until all CTAs are 7 halves of the SMs without alternatives (131072
+// fp32: 200 rows 21 us over pairs and 26 over one, 400 rows 40 and 35), 11
+// halves with few (20: 200 rows 35 us over four, 59 over one; 250 rows 52 over
+// four and 42 over pairs; 512 rows of 16384 25 over pairs, 17 over one), and
+// twice with more, whose CTAs are twice as large and merge more (128: 100 rows
+// 34 us over pairs, 42 over one; 150 rows 56 and 46).
 Plan plan_stream(const void *logits, int dtype, int rows, int vocab, long long ld, int top_k, int sms) {
   const int words = row_words(logits, dtype, vocab, ld);
   Plan p;
+  const long long most = (top_k == 0 ? 7 : top_k <= kFewTop ? 11 : 4) * sms / 2;
   p.C = 1;
-  while (p.C < 8 && (long long)rows * p.C * 2 <= 2 * sms && words / (2 * p.C) >= 512) p.C *= 2;
+  while (p.C < 8 && (long long)rows * p.C * 2 <= most && words / (2 * p.C) >= 512) p.C *= 2;
   p.wps = (words + p.C - 1) / p.C;
   p.nt = top_k <= kFewTop ? 128 : 256;
   p.even = ld * elem_size(dtype) % 16 == 0;
