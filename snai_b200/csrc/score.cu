@@ -52,6 +52,7 @@ constexpr long long kMaxElems = 1ll << 48;  // rows x stride: byte offsets stay 
 constexpr int kStages = 4;          // copy groups a row's words are committed in
 constexpr int kChunk = 4;           // words a thread takes at a time
 constexpr float kLowest = -200.f;   // exponents (base 2) are cut here: 2^-200 is 0 in fp32, and 0 * d stays 0
+constexpr double kLn2d = 0.69314718055994531;
 constexpr float kLn2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
 
 // ---- small device pieces ----
@@ -67,6 +68,10 @@ __device__ __forceinline__ float warp_max_nan(float v) {
   asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
+// The hardware's 2^x is low by this in the mean below x = -1 (measured: 2^20
+// arguments in each of four ranges down to -60 gave 4.98 to 5.16e-8; exact at
+// 0, at most 1.5e-7 off): a sum of many such terms is, and a loss takes it out.
+constexpr double kEx2Low = 5e-8;
 __device__ __forceinline__ float ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -442,6 +447,10 @@ struct Running {
       m = nm;
       most = nm + above;
     }
+    // Without W a chunk's terms are summed by themselves: fewer roundings at the
+    // sum's size, at no cost; with W the second set of sums costs 2 % (scores
+    // of 8192 x 32000 bf16 99 us for 97).
+    f2 cs = 0, cs1 = 0;
     const f2 nm2 = pack2(-m, -m), c2 = pack2(c, c), l2 = pack2(kLog2E, kLog2E);
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
@@ -458,11 +467,18 @@ struct Running {
           x = pack2(a, b);
         }
         const f2 e = pack2(ex2(a), ex2(b));
-        s = add2(s, e);
-        if (W) w = fma2(e, x, w);
-        if (S1) s1 = add2(s1, at_one<SQ>(e, d, l2));
+        if (W) {
+          s = add2(s, e);
+          w = fma2(e, x, w);
+          if (S1) s1 = add2(s1, at_one<SQ>(e, d, l2));
+        } else {
+          cs = j == 0 && k == 0 ? e : add2(cs, e);
+          if (S1) cs1 = j == 0 && k == 0 ? at_one<SQ>(e, d, l2) : add2(cs1, at_one<SQ>(e, d, l2));
+        }
       }
     }
+    if (!W) s = add2(s, cs);
+    if (!W && S1) s1 = add2(s1, cs1);
   }
   __device__ __forceinline__ Stat get() const { return {m, sum2(s), W ? sum2(w) : 0.f, S1 ? sum2(s1) : 0.f}; }
 };
@@ -499,15 +515,19 @@ struct ScoreArgs {
   Rows in;
   const int *tokens;
   int n_tok;
-  float c, inv_t;  // log2(e) / T, 1 / T
+  float c;               // log2(e) / T, rounded
+  float inv_t, inv_t_lo;  // 1 / T in two parts
+  float off;             // what c's rounding takes from log S, over W / S
   int top_k, cap, soft, grow;  // candidates: what the buffer holds (a power of two), where it is thinned out, and when
   float *logprob, *entropy;
   int *top_ids;
   float *top_logprob;
 };
 
-__device__ __forceinline__ float log_p(float z, float m, float inv_t, float s, float ls) {
-  return s == 0.f || z == -INFINITY ? -INFINITY + (s - s) : (z - m) * inv_t - ls;
+// log p of a logit; ls is log S.
+__device__ __forceinline__ float log_p(const ScoreArgs &a, float z, float m, float s, float ls) {
+  const float d = z - m;
+  return s == 0.f || z == -INFINITY ? -INFINITY + (s - s) : fmaf(d, a.inv_t, fmaf(d, a.inv_t_lo, -ls));
 }
 
 // The next float up, past both zeros.
@@ -630,21 +650,20 @@ __device__ __noinline__ int place_in_runs(const unsigned long long *cand, int n,
 // wide loads), else in sorted runs of 32 (n^2 / 5 loads, and the sorts).  The
 // whole block calls it; room for a multiple of 32.
 template <int NT>
-__device__ __forceinline__ void put_greatest(unsigned long long *cand, int n, int k, int *ids, float *lps, float m,
-                                             float inv_t, float s) {
+__device__ __forceinline__ void put_greatest(unsigned long long *cand, int n, int k, int *ids, float *lps,
+                                             const ScoreArgs &a, float m, float s, float ls) {
   const int t = threadIdx.x;
   const bool runs = n > 96;
   if (runs) {
     for (int i = t; i < (n + 31) / 32 * 32; i += NT) cand[i] = warp_sort(i < n ? cand[i] : 0);
     __syncthreads();
   }
-  const float ls = logf(s);
   for (int i = t; i < n; i += NT) {
     const unsigned long long key = cand[i];
     const int at = runs ? place_in_runs(cand, n, key) : place_by_counting(cand, n, key);
     if (at < k && key) {
       ids[at] = key_id(key);
-      lps[at] = log_p(key_logit(key), m, inv_t, s, ls);
+      lps[at] = log_p(a, key_logit(key), m, s, ls);
     }
   }
 }
@@ -806,7 +825,7 @@ __device__ __noinline__ float cut_out(const Pool p, const Slice<E, NT> s, int w0
 template <typename E, int NT, int D, bool TOPK, bool ENT>
 __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(const ScoreArgs a) {
   constexpr int NW = NT / 32, kWide = kChunk * NT, kN = Word<E>::kN;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Stat part[2][NW];
   __shared__ Slip slip[2];
   __shared__ int bound[2][NW], n_cand[2], n_ge, n_lead;
@@ -960,15 +979,17 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
     } else if (TOPK || wid * 32 < max(a.n_tok, 1)) {
       st = combine_lanes<ENT, false>(part[par][lane % NW], NW, a.c);
     }
+    // c is off by up to half a step, which is T off by as much and moves
+    // log S by that times the mean of d: known where W is
+    const float log_s = logf(st.s), ls = ENT ? fmaf(a.off, __fdividef(st.w, st.s), log_s) : log_s;
     if (rank == 0 && t < max(a.n_tok, 1)) {
-      const float ls = logf(st.s);
 #pragma unroll
       for (int i = 0; i < kMaxList / NT; ++i) {
         const int j = i * NT + t;
         if (j < a.n_tok)
-          a.logprob[(long long)r * a.n_tok + j] = in[i] ? log_p(zt[i], st.m, a.inv_t, st.s, ls) : 0.f;
+          a.logprob[(long long)r * a.n_tok + j] = in[i] ? log_p(a, zt[i], st.m, st.s, ls) : 0.f;
       }
-      if (ENT && t == 0 && a.entropy) a.entropy[r] = st.s == 0.f ? 0.f : ls - kLn2 * st.w / st.s;
+      if (ENT && t == 0 && a.entropy) a.entropy[r] = st.s == 0.f ? 0.f : log_s - kLn2 * st.w / st.s;
     }
     if (TOPK) {
       int *ids = a.top_ids + (long long)r * a.top_k;
@@ -977,7 +998,7 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
         if (rank == 0)
           for (int i = t; i < a.top_k; i += NT) ids[i] = -1, lps[i] = NAN;
       } else if (C == 1) {
-        put_greatest<NT>(cand, n, a.top_k, ids, lps, st.m, a.inv_t, st.s);
+        put_greatest<NT>(cand, n, a.top_k, ids, lps, a, st.m, st.s, ls);
       } else {
         const uint32_t to_n = mapa_shared(smem_u32(&n_lead), 0), to = mapa_shared(smem_u32(gath), 0);
         const uint32_t to_ge = mapa_shared(smem_u32(&n_ge), 0);
@@ -1014,7 +1035,7 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
           gather();
           cluster_sync_all();
         }
-        if (rank == 0) put_greatest<NT>(gath, m, a.top_k, ids, lps, st.m, a.inv_t, st.s);
+        if (rank == 0) put_greatest<NT>(gath, m, a.top_k, ids, lps, a, st.m, st.s, ls);
       }
     }
     if (r + step < a.in.rows) cur.next(a.in, r, step, rank);
@@ -1033,6 +1054,10 @@ struct RowGradArgs {
   float c;           // log2(e) / T
   float inv_t_f;
   double inv_t;      // 1 / T
+  // the 1 / T that c, rounded, stands for, and the 1 that a label's exponents
+  // do: with them a loss is that of a temperature off by half a step of fp32,
+  // and not the difference of two
+  double inv_t_z, one_z;
   const float *g_entropy;
   const int *labels;
   const float *row_grad;
@@ -1108,7 +1133,9 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
   constexpr int NW = NT / 32, kN = Word<E>::kN, kWide = kChunk * NT;
   constexpr bool ENT = MODE == 0 && EXTRA, LABEL1 = MODE == 1 && EXTRA;
   constexpr int SQ = LABEL1 ? EXTRA - 1 : 0;  // squarings that make exp(d) of exp(d / T)
-  extern __shared__ __align__(16) unsigned char smem[];
+  // aligned: else a warp's 512 bytes take five rows of banks (2048 x 131072
+  // with the rest 376 us, and 435 on 16 bytes)
+  extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Stat part[2][NW], listed[2][kMaxEntryWarps];
   // by entry warp: the sums of q (MODE 0: g) and of q (log q - (z - top) / T), and top
   __shared__ double sum_q[2][kMaxEntryWarps], sum_kl[kMaxEntryWarps];
@@ -1268,9 +1295,11 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
           if (valid(ids[j])) tm = max_nan(tm, vals[j]);
         tm = warp_max_nan(tm);
         for (int j = lane; j < n; j += 32)
-          if (valid(ids[j]) && vals[j] != -INFINITY) s += expf((vals[j] - tm) * a.inv_t_f);
+          if (valid(ids[j]) && vals[j] != -INFINITY) s += expf((float)(((double)vals[j] - tm) * a.inv_t));
         s = warp_sum(s);
-        lse = tm == -INFINITY ? 0.0 : tm * a.inv_t + (double)logf(s);
+        // log s = ls + log(s exp(-ls)), the second to its first order: an error here is one of the whole loss
+        const float ls = logf(s);
+        lse = tm == -INFINITY ? 0.0 : tm * a.inv_t + ls + ((double)s * exp_d(-(double)ls) - 1.0);
       }
       for (int j = et; j < ne; j += nte) zl[j] = j == et ? z0 : valid(ids[j]) ? Word<E>::one(cur.at(ids[j])) : -INFINITY;
       // logits are taken relative to the warp's greatest, so that a row of the type's lowest values keeps its differences
@@ -1292,7 +1321,7 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
         } else if (valid(id) && vals[j] != -INFINITY) {
           const double lq = rest ? (double)vals[j] : vals[j] * a.inv_t - lse;
           q = exp_d(lq);  // not fp32's: an entry of 1e-60 against a masked logit is an infinite loss all the same
-          if (q != 0.0) kl_own += q * (lq - ((double)z - top) * a.inv_t);
+          if (q != 0.0) kl_own += q * (lq - ((double)z - top) * a.inv_t_z);
         }
         q_own += q;
         wt[j] = (float)q;
@@ -1350,13 +1379,13 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
           if (S == 0.f) {
             l = q_all > 0 ? INFINITY : 0.0;
           } else {
-            for (int w = 0; w < nwe; ++w) l += sum_kl[w] + sum_q[par][w] * (((double)m - list_top[w]) * a.inv_t);
-            l += q_all * log((double)S);
-            if (rr > 0.0) l += rr * (log(rr) + log1p((double)lst.s / unlisted));
+            for (int w = 0; w < nwe; ++w) l += sum_kl[w] + sum_q[par][w] * (((double)m - list_top[w]) * a.inv_t_z);
+            l += q_all * (log((double)S) + kEx2Low * (1.0 - inv_s));
+            if (rr > 0.0) l += rr * (log(rr) + log1p((double)lst.s / unlisted) - kEx2Low * inv_s);
           }
           l *= (1.0 - a.a) * a.t * a.t;
         }
-        if (y >= 0) l += a.a * (label_z == -INFINITY ? INFINITY : (double)m - label_z + log((double)S1));
+        if (y >= 0) l += a.a * (label_z == -INFINITY ? INFINITY : ((double)m - label_z) * a.one_z + log((double)S1));
         a.loss[r] = !any ? 0.f : S != S ? NAN : (float)l;
       }
       for (int j = et; j < ne; j += nte)
@@ -1765,7 +1794,11 @@ int launch_score(const char *who, const ScoreLaunch &s, cudaStream_t stream) {
   a.tokens = s.tokens;
   a.n_tok = s.n_tok;
   a.c = (float)(1.4426950408889634 / s.temperature);
-  a.inv_t = (float)(1.0 / s.temperature);
+  const bool ent = s.top_k > 0 || s.entropy;  // W is at hand
+  const double inv = ent ? 1.0 / s.temperature : kLn2d * a.c;
+  a.inv_t = (float)inv;
+  a.inv_t_lo = (float)(inv - a.inv_t);
+  a.off = ent ? (float)(1.0 / s.temperature / a.c - kLn2d) : 0.f;
   a.top_k = s.top_k;
   a.logprob = s.logprob;
   a.entropy = s.entropy;
@@ -1847,7 +1880,9 @@ int launch_distill(const char *who, const DistillLaunch &s, cudaStream_t stream)
   a.loss = s.loss;
   a.grad = s.grad;
   a.grad_ld = s.grad_ld;
+  a.inv_t_z = kLn2d * a.c;
   const int extra = !labels || s.temperature == 1.0 ? 0 : s.temperature == 2.0 ? 2 : s.temperature == 4.0 ? 3 : 1;
+  a.one_z = kLn2d * (extra == 1 ? (double)kLog2E : a.c * s.temperature);  // the powers are of c's exponents
   return launch_row_grad(who, a, s.dtype, 1, extra, dev, stream);
 }
 
