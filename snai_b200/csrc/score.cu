@@ -19,12 +19,12 @@
 // cut into slices over a cluster of CTAs when it is long.
 //
 // Measured on a B200 against its copy rate of 6553 GB/s (the bytes each
-// operator cannot do without over its time): 8192 x 16384 fp32 scores 0.91,
-// with 20 alternatives 0.60, gradient 0.87, distillation of 64 entries with
-// labels 0.78; 8192 x 32000 bf16 scores 0.82, 2048 x 131072 bf16 gradient 0.78
-// (issue-bound: 11 lane instructions for two bytes of an element; an eighth or
-// a quarter of the exponentials on the FMA pipe made it slower); 2048 x 131072
-// fp32 scores 0.95, with 64 alternatives 0.73, distillation with the rest 0.75.
+// operator cannot do without over its time): 2048 x 131072 fp32 scores 0.98,
+// with 64 alternatives 0.71, distillation with the rest 0.87; 8192 x 16384
+// fp32 scores with 20 alternatives 0.58, gradient 0.83, distillation of 64
+// entries with labels 0.86; 8192 x 32000 bf16 scores 0.83, 2048 x 131072 bf16
+// gradient 0.79 (issue-bound: 11 lane instructions for two bytes of an element;
+// an eighth or a quarter of the exponentials on the FMA pipe made it slower).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -1108,8 +1108,8 @@ __device__ __forceinline__ void cluster_meet() {
 //   grad_i = e_i alpha + gamma softmax(z)_i - what the list and the label take.
 // EXTRA: labels at T != 1, whose softmax needs exponentials of its own (1), or
 // at T = 2 or 4 the squares (2) or fourth powers (3) of those at hand
-// (16384 x 8192, 64 entries: 211 us against 225 with exponentials of their
-// own; 4096 x 32000 bf16: 135 against 169).  With `rest` the listed logits
+// (8192 x 16384, 64 entries: 192 us against 215 with exponentials of their
+// own; 4096 x 32000 bf16: 133 against 169).  With `rest` the listed logits
 // are taken out of the staged row (each by the thread that owns its word,
 // which finds it in a list of its own), so that the unlisted mass is a sum of
 // its own: 1 - the listed would lose a confident student's.
@@ -1121,7 +1121,7 @@ __device__ __forceinline__ void cluster_meet() {
 // out.  Pass B writes the terms that every element has; the entries' ids get
 // theirs from the entry threads one row later, behind the next row's barrier,
 // when all owners have written the base.  (Entries held by threads that also
-// take the row took 46 us where this takes 34, at 1024 x 16384 with 64 entries
+// take the row took 46 us where these took 34, at 1024 x 16384 with 64 entries
 // and labels: their chain of dependent steps is as long as both passes.)  An
 // id listed more than once is handled by its first entry, in the order of the
 // list: no atomics.  The entries' weights and the loss are held in 64 bits: a
