@@ -19,7 +19,7 @@
 // cut into slices over a cluster of CTAs when it is long.
 //
 // Measured on a B200 against its copy rate of 6553 GB/s (the bytes each
-// operator cannot do without over its time): 2048 x 131072 fp32 scores 0.98,
+// operator cannot do without over its time): 2048 x 131072 fp32 scores 1.04,
 // with 64 alternatives 0.71, distillation with the rest 0.87; 8192 x 16384
 // fp32 scores with 20 alternatives 0.58, gradient 0.83, distillation of 64
 // entries with labels 0.86; 8192 x 32000 bf16 scores 0.83, 2048 x 131072 bf16
@@ -1618,7 +1618,7 @@ int row_words(const void *logits, int dtype, int vocab, long long ld) {
 // short of CTAs a row is spread over a cluster of up to 8, down to slices of
 // 8 KB: until all CTAs are 7 halves of the SMs without alternatives (131072
 // fp32: 200 rows 21 us over pairs and 26 over one, 400 rows 40 and 35), 11
-// halves with few (20: 200 rows 35 us over four, 59 over one; 250 rows 52 over
+// halves with few (these with three chunks in flight; 20: 200 rows 35 us over four, 59 over one; 250 rows 52 over
 // four and 42 over pairs; 512 rows of 16384 25 over pairs, 17 over one), and
 // twice with more, whose CTAs are twice as large and merge more (128: 100 rows
 // 34 us over pairs, 42 over one; 150 rows 56 and 46).
@@ -1713,7 +1713,10 @@ int by_dtype(int dtype, F &&f) {
   return f(__half());
 }
 
-constexpr int kRing128 = 3, kRing256 = 4;  // chunks in flight a CTA
+// Chunks in flight a CTA.  One more each left a CTA less an SM: 301 rows of
+// 50001 fp16 with 128 alternatives 38 us for 27, 2048 x 131072 fp32 without
+// 167 for 157; only calls of few CTAs would gain (200 such rows 21 for 24).
+constexpr int kRing128 = 2, kRing256 = 3;
 
 template <typename E, int NT, int D>
 int score_nt(const char *who, const ScoreArgs &a, size_t smem, int dev, cudaStream_t st) {
