@@ -828,7 +828,8 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Stat part[2][NW];
   __shared__ Slip slip[2];
-  __shared__ int bound[2][NW], n_cand[2], n_ge, n_lead;
+  __shared__ int bound[2][NW], n_cand[2], n_ge;
+  __shared__ int n_lead[2];  // by row: the others read a row's count while rank 0 is already at the next one
   uint4 *ring = reinterpret_cast<uint4 *>(smem);
   // candidates, then (rank 0 of a cluster) those of all slices
   unsigned long long *cand = reinterpret_cast<unsigned long long *>(smem + D * kWide * 16);
@@ -967,7 +968,7 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
         if (TOPK)
           tau = st.s != st.s ? INFINITY
                              : about_kth(cand, n, (a.top_k + C - 1) / C);
-        if (lane == 0) slip[par].st = st, slip[par].tau = tau, n_lead = 0;
+        if (lane == 0) slip[par].st = st, slip[par].tau = tau, n_lead[par] = 0;
       }
       cluster_sync_all();
       const bool on = lane % 16 < C;
@@ -1000,7 +1001,7 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
       } else if (C == 1) {
         put_greatest<NT>(cand, n, a.top_k, ids, lps, a, st.m, st.s, ls);
       } else {
-        const uint32_t to_n = mapa_shared(smem_u32(&n_lead), 0), to = mapa_shared(smem_u32(gath), 0);
+        const uint32_t to_n = mapa_shared(smem_u32(&n_lead[par]), 0), to = mapa_shared(smem_u32(gath), 0);
         const uint32_t to_ge = mapa_shared(smem_u32(&n_ge), 0);
         unsigned long long lo = sort_key(tau, INT_MAX), hi = ~0ull;
         auto gather = [&] {
@@ -1017,7 +1018,7 @@ __global__ void __launch_bounds__(NT, (NT == 128 ? 8 : 4) - TOPK) snai_score(con
           while (lo < hi) {
             const unsigned long long mid = lo + ((hi - lo - 1) >> 1) + 1;
             cluster_sync_all();
-            if (t == 0) n_ge = 0, n_lead = 0;
+            if (t == 0) n_ge = 0, n_lead[par] = 0;
             cluster_sync_all();
             int g = 0;
             for (int i = t; i < n; i += NT) g += cand[i] >= mid;
