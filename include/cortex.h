@@ -432,7 +432,9 @@ CORTEX_API int cortex_score_grad(const void *logits, int dtype, int rows, int vo
  *   temperature already (cortex_score's top_logprob): q = exp(teacher_logits),
  *   and what the list leaves of 1 (at least 0) is one more outcome, set
  *   against the student's probability of all unlisted ids.  Where the student
- *   has none (every unlisted id masked) that outcome is left out.
+ *   has none, that outcome is left out: every unlisted id is masked, by -inf
+ *   or by a finite value so low that their probability is below e^-745 (0 in
+ *   64 bits).
  * A listed q of 0 (below e^-700) adds nothing; any other against a masked
  * logit makes the loss infinite.  A row whose list and label are all padding
  * has loss 0 and gradient 0, whatever its logits hold. */

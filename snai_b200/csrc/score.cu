@@ -1128,6 +1128,7 @@ __device__ __forceinline__ void cluster_meet() {
 // list: no atomics.  The entries' weights and the loss are held in 64 bits: a
 // handful of values a row, and a loss that is a small difference of large
 // terms.
+constexpr float kNoRest = 1074.8f;  // 745 / ln 2: e^-745 is the least number of 64 bits
 constexpr int kMaxEntryWarps = 2;  // more would cost the third CTA of an SM its registers
 template <typename E, int NT, int MODE, int EXTRA>
 __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) snai_row_grad(const RowGradArgs a) {
@@ -1190,10 +1191,13 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
   __syncthreads();
   int par = 0;
 
-  // The scalars of a row, by every warp behind the row's barrier.
-  float m, S, S1, unlisted, inv_s, inv_s1, alpha, beta, gamma, kt, ky, mass, ru;
+  // The scalars of a row, by every warp behind the row's barrier.  S and S1 are
+  // relative to m.  With `rest` the unlisted sum su is relative to the unlisted
+  // maximum mu, and stays so: relative to a listed one 87 T above it would be 0.
+  // Pass B, which then gives the unlisted ids' gradients alone, takes its
+  // exponentials relative to mu too (else mu is m).
+  float m, mu, S, S1, su, inv_s, inv_s1, alpha, beta, gamma, kt, ky, mass, rest_k;
   double rr, q_all;
-  Stat lst;
   auto scalars = [&](float sc, int y) {
     Stat st = combine_lanes<ENT, LABEL1>(part[par][lane % NW], NW, a.c);
     if (C > 1) {
@@ -1207,37 +1211,44 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
     }
     q_all = sum_q[par][0];
     if (nwe > 1) q_all += sum_q[par][1];
-    lst = no_stat();
+    mu = st.m, su = st.s;
+    float f = 1.f;  // 2^((mu - m) c)
     if (rest) {
-      if (lane % 2 < nwe) lst = listed[par][lane % 2];
-      const float both = max_nan(st.m, warp_max_nan(lst.m));
-      rebase<false, LABEL1>(st, both, a.c);
+      Stat lst = lane % 2 < nwe ? listed[par][lane % 2] : no_stat();
+      const float both = max_nan(mu, warp_max_nan(lst.m));
+      f = ex2(cut((mu - both) * a.c));
+      if (LABEL1) st.s1 *= ex2(cut((mu - both) * kLog2E));
       rebase<false, LABEL1>(lst, both, a.c);
       lst = combine_lanes<false, LABEL1>(lst, 2, a.c);
+      st.m = both;
+      st.s = fmaf(su, f, lst.s);
+      if (LABEL1) st.s1 += lst.s1;
     }
     m = st.m;
-    S = st.s + lst.s;
-    S1 = LABEL1 ? st.s1 + lst.s1 : S;
+    S = st.s;
+    S1 = LABEL1 ? st.s1 : S;
     inv_s = S == 0.f ? 0.f : 1.f / S;
     inv_s1 = LABEL1 ? (S1 == 0.f ? 0.f : 1.f / S1) : inv_s;
-    unlisted = beta = gamma = kt = ky = mass = ru = 0.f;
+    beta = gamma = kt = ky = mass = rest_k = 0.f;
     rr = 0;
     if (MODE == 0) {
       const float gh = ENT ? sc : 0.f, k = inv_s * a.inv_t_f;
       alpha = -(float)q_all * k;
       if (ENT) alpha += gh * kLn2 * st.w * inv_s * k, beta = -gh * kLn2 * k;
     } else {
-      rr = rest && st.s > 0.f ? fmax(0.0, 1.0 - q_all) : 0.0;
+      bool none = su == 0.f;  // of the student's unlisted probability is there in 64 bits (su is 0 or at least 1)
+      if (rest && f == 0.f) none = none || !((m - mu) * a.c + (__log2f(S) - __log2f(su)) < kNoRest);
+      rr = rest && !none ? fmax(0.0, 1.0 - q_all) : 0.0;
       mass = (float)(q_all + rr);
-      unlisted = st.s;
-      ru = rr > 0.0 ? (float)rr * (S / st.s) : 0.f;  // the teacher's rest over the student's
+      rest_k = rr > 0.0 ? (float)rr / su : 0.f;  // times an unlisted e_i: what the teacher's rest gives to i
       kt = sc * (float)((1.0 - a.a) * a.t);
       ky = y >= 0 ? sc * (float)a.a : 0.f;
-      alpha = kt * (mass - ru) * inv_s;
+      f *= inv_s;  // times e_i: p_i
+      alpha = kt * (mass * f - rest_k);
       if (LABEL1)
-        gamma = ky * inv_s1;
+        gamma = ky * (rest ? ex2(cut((mu - m) * kLog2E)) * inv_s1 : inv_s1);
       else
-        alpha += ky * inv_s;
+        alpha += ky * f;
     }
   };
 
@@ -1364,7 +1375,7 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
             g = ex2(x) * fmaf(x, beta, alpha) + q * a.inv_t_f;
           } else {
             const float p = ex2(cut(d * a.c)) * inv_s;
-            g = kt * (j < n ? mass * p - q : (mass - ru) * p);
+            g = kt * (mass * p - (j < n ? q : rest_k * ex2(cut((z - mu) * a.c))));
             if (y >= 0) {
               const float p1 = LABEL1 ? ex2(cut(d * kLog2E)) * inv_s1 : p;
               g += ky * (id == y ? p1 - 1.f : p1);
@@ -1374,20 +1385,34 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
         }
         before = static_cast<E *>(a.grad) + (long long)r * a.grad_ld;
       }
-      if (MODE == 1 && et == nte - 32 && rank == 0) {
+      if (MODE == 1 && et >= nte - 32 && rank == 0) {  // the loss, by the last entry warp
+        Stat lst = no_stat();
+        if (rest) lst = combine_lanes<false, false>(lane % 2 < nwe ? listed[par][lane % 2] : no_stat(), 2, a.c);
+        // With `rest` S is taken again in 64 bits from its two parts, relative to
+        // the greater one's maximum: no gap between them is lost, and log S and
+        // the log of the unlisted sum come from the same terms.
+        const bool parts = rest && su > 0.f, above = parts && lst.m > mu;
+        const double g = parts ? ((double)lst.m - mu) * a.inv_t_z : 0.0, x = exp_d(-fabs(g));
+        const double all = !parts ? (double)S : above ? lst.s + x * su : su + x * lst.s;
+        // every logarithm at once, a lane each
+        const double logs = log(lane == 0 ? all : lane == 1 ? (double)su : lane == 2 ? (double)S1 : rr);
+        auto log_of = [&](int i) { return __shfl_sync(0xffffffffu, logs, i); };
         double l = 0;
-        if (a.a < 1.0) {
-          if (S == 0.f) {
-            l = q_all > 0 ? INFINITY : 0.0;
-          } else {
-            for (int w = 0; w < nwe; ++w) l += sum_kl[w] + sum_q[par][w] * (((double)m - list_top[w]) * a.inv_t_z);
-            l += q_all * (log((double)S) + kEx2Low * (1.0 - inv_s));
-            if (rr > 0.0) l += rr * (log(rr) + log1p((double)lst.s / unlisted) - kEx2Low * inv_s);
-          }
-          l *= (1.0 - a.a) * a.t * a.t;
+        if (S == 0.f) {
+          l = q_all > 0 ? INFINITY : 0.0;
+        } else {
+          // the terms that are exact, one in each part
+          const float tops = parts && lst.s > 0.f ? 1.f + (float)x : 1.f;
+          const double log_s = log_of(0) + kEx2Low * (1.f - __fdividef(tops, (float)all));
+          if (rr > 0.0)  // the student's rest is the unlisted sum over all
+            l = rr * (log_of(3) + (log_s - (log_of(1) + kEx2Low * (1.f - __fdividef(1.f, su)))) + (above ? g : 0.0));
+          const double ref = !parts ? m : above ? lst.m : mu;  // what log_s is relative to
+          for (int w = 0; w < nwe; ++w) l += sum_kl[w] + sum_q[par][w] * ((ref - list_top[w]) * a.inv_t_z);
+          l += q_all * log_s;
         }
-        if (y >= 0) l += a.a * (label_z == -INFINITY ? INFINITY : ((double)m - label_z) * a.one_z + log((double)S1));
-        a.loss[r] = !any ? 0.f : S != S ? NAN : (float)l;
+        l = a.a < 1.0 ? l * ((1.0 - a.a) * a.t * a.t) : 0.0;
+        if (y >= 0) l += a.a * (label_z == -INFINITY ? INFINITY : ((double)m - label_z) * a.one_z + log_of(2));
+        if (lane == 0) a.loss[r] = !any ? 0.f : S != S ? NAN : (float)l;
       }
       for (int j = et; j < ne; j += nte)
         if (valid(ids[j])) head[hash(ids[j])] = -1;
@@ -1449,7 +1474,7 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
         // pass B
         E *out = static_cast<E *>(a.grad) + (long long)r * a.grad_ld;
         const bool vec = ((reinterpret_cast<uintptr_t>(out) + (long long)cur.base * (int)sizeof(E)) & 15) == 0;
-        const f2 nm2 = pack2(-m, -m), c2 = pack2(a.c, a.c), l2 = pack2(kLog2E, kLog2E);
+        const f2 nm2 = pack2(-mu, -mu), c2 = pack2(a.c, a.c), l2 = pack2(kLog2E, kLog2E);
         const f2 al2 = pack2(alpha, alpha), be2 = pack2(beta, beta), ga2 = pack2(gamma, gamma);
 #pragma unroll 1
         for (int s = 0; s < kStages; ++s) {
