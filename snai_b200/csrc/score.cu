@@ -516,7 +516,7 @@ struct ScoreArgs {
   const int *tokens;
   int n_tok;
   float c;               // log2(e) / T, rounded
-  float inv_t, inv_t_lo;  // 1 / T in two parts
+  float two_t, two_t_lo;  // 2 / T in two parts
   float off;             // what c's rounding takes from log S, over W / S
   int top_k, cap, soft, grow;  // candidates: what the buffer holds (a power of two), where it is thinned out, and when
   float *logprob, *entropy;
@@ -524,10 +524,12 @@ struct ScoreArgs {
   float *top_logprob;
 };
 
-// log p of a logit; ls is log S.
+// log p of a logit; ls is log S.  Half the difference never passes fp32's
+// range, where the difference of logits at both of its ends would: over T it
+// may be back inside.
 __device__ __forceinline__ float log_p(const ScoreArgs &a, float z, float m, float s, float ls) {
-  const float d = z - m;
-  return s == 0.f || z == -INFINITY ? -INFINITY + (s - s) : fmaf(d, a.inv_t, fmaf(d, a.inv_t_lo, -ls));
+  const float d = fmaf(0.5f, z, -0.5f * m);
+  return s == 0.f || z == -INFINITY ? -INFINITY + (s - s) : fmaf(d, a.two_t, fmaf(d, a.two_t_lo, -ls));
 }
 
 // The next float up, past both zeros.
@@ -1825,8 +1827,8 @@ int launch_score(const char *who, const ScoreLaunch &s, cudaStream_t stream) {
   a.c = (float)(1.4426950408889634 / s.temperature);
   const bool ent = s.top_k > 0 || s.entropy;  // W is at hand
   const double inv = ent ? 1.0 / s.temperature : kLn2d * a.c;
-  a.inv_t = (float)inv;
-  a.inv_t_lo = (float)(inv - a.inv_t);
+  a.two_t = (float)(2.0 * inv);
+  a.two_t_lo = (float)(2.0 * inv - a.two_t);
   a.off = ent ? (float)(1.0 / s.temperature / a.c - kLn2d) : 0.f;
   a.top_k = s.top_k;
   a.logprob = s.logprob;
