@@ -40,6 +40,17 @@ class Score(NamedTuple):
     top_logprob: Any = None
 
 
+_INT_MAX = (1 << 31) - 1
+
+
+def _c_int(name, v):
+    """v as an int of the C interface, which would take it modulo 2^32."""
+    v = int(v)
+    if v > _INT_MAX or v < -_INT_MAX:
+        raise CortexError(f"{name} {v} does not fit an int")
+    return v
+
+
 def _ptr(a):
     return a.ctypes.data_as(ctypes.c_void_p)
 
@@ -148,7 +159,7 @@ class Cortex:
         sl = None if slots is None else np.ascontiguousarray(slots, dtype=np.int32)
         if sl is not None and len(sl) != B:
             raise CortexError(f"{len(sl)} slots for {B} rows of tokens")
-        k = int(top_k)
+        k = _c_int("top_k", top_k)
         lp = None if tg is None else np.zeros((B, n), dtype=np.float32)
         ent = np.zeros((B, n), dtype=np.float32)
         ids = np.full((B, n, k), -1, dtype=np.int32) if k > 0 else None
@@ -381,6 +392,8 @@ def _dev_rows(logits):
         raise CortexError(f"logits must be a 2-d CUDA tensor of float32, bfloat16 or float16, got {logits.dtype} "
                           f"{tuple(logits.shape)} on {logits.device}")
     rows, vocab = logits.shape
+    if rows > _INT_MAX or vocab > _INT_MAX:
+        raise CortexError(f"logits {tuple(logits.shape)}: a size does not fit an int")
     ld, one = logits.stride()
     if one != 1 and vocab > 1:
         raise CortexError("the elements of a row of logits must be adjacent")
@@ -405,7 +418,7 @@ def _dev_tokens(tokens, logits, rows, dtype):
         return _dev_arg("tokens", tokens, logits, (rows,), dtype), 1
     if tokens.dim() != 2:
         raise CortexError("tokens must be [rows] or [rows, n]")
-    return _dev_arg("tokens", tokens, logits, (rows, tokens.shape[1]), dtype), tokens.shape[1]
+    return _dev_arg("tokens", tokens, logits, (rows, tokens.shape[1]), dtype), _c_int("tokens a row", tokens.shape[1])
 
 
 def _on(stream, device, torch, made):
@@ -435,7 +448,7 @@ def score_device(logits_dev, tokens_dev=None, temperature=1.0, top_k=0, want_ent
     torch = _torch()
     code, rows, vocab, ld = _dev_rows(logits_dev)
     tok, n = _dev_tokens(tokens_dev, logits_dev, rows, torch.int32)
-    k = int(top_k)
+    k = _c_int("top_k", top_k)
     new, f32 = logits_dev.new_empty, torch.float32
 
     def made():
@@ -482,7 +495,7 @@ def distill_device(logits_dev, teacher_ids_dev, teacher_logits_dev, labels=None,
     code, rows, vocab, ld = _dev_rows(logits_dev)
     if teacher_ids_dev.dim() != 2:
         raise CortexError("teacher_ids must be [rows, k]")
-    k, f32 = teacher_ids_dev.shape[1], torch.float32
+    k, f32 = _c_int("teacher entries", teacher_ids_dev.shape[1]), torch.float32
     ids = _dev_arg("teacher_ids", teacher_ids_dev, logits_dev, (rows, k), torch.int32)
     vals = _dev_arg("teacher_logits", teacher_logits_dev, logits_dev, (rows, k), f32)
     y = _dev_arg("labels", labels, logits_dev, (rows,), torch.int32)
