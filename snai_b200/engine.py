@@ -251,8 +251,10 @@ class Cortex:
         ids = np.ascontiguousarray(teacher_ids, dtype=np.int32)
         vals = np.ascontiguousarray(teacher_logits, dtype=np.float32)
         y = None if labels is None else np.ascontiguousarray(labels, dtype=np.int32)
-        if ids.ndim != 2 or ids.shape != vals.shape or len(ids) != len(a) or (y is not None and len(y) != len(a)):
-            raise CortexError(f"inputs {a.shape}, teacher lists {ids.shape} / {vals.shape} and labels do not match")
+        if a.ndim != 1 or ids.ndim != 2 or ids.shape != vals.shape or len(ids) != len(a) or (
+                y is not None and y.shape != a.shape):
+            raise CortexError(f"inputs {a.shape}, teacher lists {ids.shape} / {vals.shape} and labels "
+                              f"{None if y is None else y.shape} do not match")
         prm = distill_params(temperature, label_weight, rest)
         loss = ctypes.c_float(0.0)
         check(self.lib.cortex_distill_grads(self.h, _ptr(a), _ptr(ids), _ptr(vals), ids.shape[1],

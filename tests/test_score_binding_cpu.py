@@ -1,5 +1,6 @@
 """What the Python binding of the vocabulary-row operators refuses by itself:
-sizes that an int of the C interface would take modulo 2^32."""
+sizes that an int of the C interface would take modulo 2^32, and lists,
+labels and inputs of a distillation step that do not go together."""
 import numpy as np
 import pytest
 
@@ -43,3 +44,21 @@ def test_alternatives_past_an_int_are_refused(k):
     state.lib = state.h = None
     with pytest.raises(CortexError, match="top_k"):
         state.score(np.ones((1, 3), dtype=np.int32), None, 1.0, k)
+
+
+@pytest.mark.parametrize("inputs,ids,vals,labels", [
+    ((5,), (5, 3), (5, 3), (5, 2)),  # two labels a position
+    ((5,), (5, 3), (5, 3), (4,)),
+    ((5, 2), (5, 3), (5, 3), None),  # two inputs a position
+    ((1, 5), (5, 3), (5, 3), None),
+    ((5,), (5,), (5,), None),
+    ((5,), (5, 3), (5, 2), None),
+    ((5,), (4, 3), (4, 3), None),
+], ids=str)
+def test_distillation_arrays_go_together(inputs, ids, vals, labels):
+    state = object.__new__(Cortex)
+    state.lib = state.h = None
+    with pytest.raises(CortexError, match="do not match"):
+        state.distill_grads(np.ones(inputs, dtype=np.int32), np.ones(ids, dtype=np.int32),
+                            np.zeros(vals, dtype=np.float32), None if labels is None else np.ones(labels, dtype=np.int32),
+                            1.0, 0.0 if labels is None else 0.5)
