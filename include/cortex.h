@@ -380,7 +380,8 @@ CORTEX_API int cortex_train_info(void *state, int *adam_steps, float *clip_facto
 /*                                                                           */
 /* logits[rows][ld] (row stride ld >= vocab, vocab <= 524288, rows <= 2^30,  */
 /* rows * ld <= 2^48) are fp32, bf16 or fp16; any alignment of the rows to   */
-/* an element is taken, 16-byte aligned rows are fastest.  Within a row,     */
+/* an element is taken, 16-byte aligned rows are fastest; all other arrays   */
+/* are aligned to 4 bytes.  Within a row,                                    */
 /* p = softmax(logits / temperature), 0.001 <= temperature <= 1000.          */
 /* Statistics are held in fp32 or more.                                      */
 /*  - An id outside [0, vocab) is padding: log probability 0, no teacher     */

@@ -1574,6 +1574,17 @@ int elem_size(int dtype) { return dtype == SNAI_DTYPE_FP32 ? 4 : 2; }
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// Ids and floats are read and written by fours of bytes: an odd address is an
+// error here instead of one of the GPU's.  (Host arrays may lie anywhere.)
+int check_words(const char *who, std::initializer_list<std::pair<const char *, const void *>> ptrs) {
+  for (const auto &p : ptrs)
+    if (!aligned(p.second, 4)) {
+      set_error("%s: %s is not aligned to 4 bytes", who, p.first);
+      return -2;
+    }
+  return 0;
+}
+
 // What every call of this file checks of its rows and temperature.
 int check_rows(const char *who, const void *logits, int dtype, int rows, int vocab, long long ld, double t) {
   if (dtype != SNAI_DTYPE_FP32 && dtype != SNAI_DTYPE_BF16 && dtype != SNAI_DTYPE_FP16) {
@@ -1812,7 +1823,13 @@ int check_score(const char *who, const ScoreLaunch &s) {
 }
 
 int launch_score(const char *who, const ScoreLaunch &s, cudaStream_t stream) {
-  const int rc = check_score(who, s);
+  int rc = check_score(who, s);
+  if (rc == 0)
+    rc = check_words(who, {{"tokens", s.tokens},
+                           {"logprob", s.logprob},
+                           {"entropy", s.entropy},
+                           {"top_ids", s.top_ids},
+                           {"top_logprob", s.top_logprob}});
   if (rc) return rc;
   if (s.rows == 0) return 0;
   const bool tok = s.n_tok > 0, top = s.top_k > 0;
@@ -1885,7 +1902,13 @@ int check_distill(const char *who, const DistillLaunch &s) {
 }
 
 int launch_distill(const char *who, const DistillLaunch &s, cudaStream_t stream) {
-  const int rc = check_distill(who, s);
+  int rc = check_distill(who, s);
+  if (rc == 0)
+    rc = check_words(who, {{"teacher_ids", s.teacher_ids},
+                           {"teacher_logits", s.teacher_logits},
+                           {"labels", s.labels},
+                           {"row_grad", s.row_grad},
+                           {"loss", s.loss}});
   if (rc) return rc;
   if (s.rows == 0) return 0;
   const int *labels = s.label_weight > 0.0 ? s.labels : nullptr;
@@ -1965,7 +1988,8 @@ extern "C" int cortex_score_grad(const void *logits, int dtype, int rows, int vo
     set_error("%s: NULL grad, tokens or g_logprob", who);
     return -2;
   }
-  rc = check_grad(who, logits, dtype, rows, vocab, ld, grad, grad_ld);
+  rc = check_words(who, {{"tokens", tokens}, {"g_logprob", g_logprob}, {"g_entropy", g_entropy}});
+  if (rc == 0) rc = check_grad(who, logits, dtype, rows, vocab, ld, grad, grad_ld);
   if (rc) return rc;
   if (rows == 0) return 0;
   if (n_tok == 0) tokens = nullptr, g_logprob = nullptr;

@@ -1,12 +1,16 @@
-"""What the Python binding of the vocabulary-row operators refuses by itself:
+"""More refusals of the vocabulary-row operators, the Python binding's own first:
 sizes that an int of the C interface would take modulo 2^32, and lists,
-labels and inputs of a distillation step that do not go together."""
+labels and inputs of a distillation step that do not go together; then
+addresses that the GPU cannot read."""
+import ctypes
+
 import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 
 from snai_b200 import Cortex, CortexError, distill_device, score_device, score_grad_device  # noqa: E402
+from test_score_cpu import distill, score, score_grad  # noqa: E402
 
 
 class Rows:
@@ -62,3 +66,21 @@ def test_distillation_arrays_go_together(inputs, ids, vals, labels):
         state.distill_grads(np.ones(inputs, dtype=np.int32), np.ones(ids, dtype=np.int32),
                             np.zeros(vals, dtype=np.float32), None if labels is None else np.ones(labels, dtype=np.int32),
                             1.0, 0.0 if labels is None else 0.5)
+
+
+ODD = ctypes.c_void_p((1 << 21) + 2)
+
+
+@pytest.mark.parametrize("call,name,kw", [
+    (score, "tokens", dict(tokens=ODD)), (score, "logprob", dict(lp=ODD)), (score, "entropy", dict(ent=ODD)),
+    (score, "top_ids", dict(ids=ODD)), (score, "top_logprob", dict(top=ODD)),
+    (score_grad, "tokens", dict(tokens=ODD)), (score_grad, "g_logprob", dict(gl=ODD)),
+    (score_grad, "g_entropy", dict(gh=ODD)),
+    (distill, "teacher_ids", dict(ids=ODD)), (distill, "teacher_logits", dict(vals=ODD)),
+    (distill, "labels", dict(labels=ODD, a=0.5)), (distill, "row_grad", dict(rg=ODD)), (distill, "loss", dict(loss=ODD)),
+], ids=str)
+def test_odd_addresses_are_refused(built, call, name, kw):
+    """They would fault the GPU."""
+    from snai_b200 import last_error, load
+    assert call(load(), **kw) == -2
+    assert name in last_error() and "aligned" in last_error()
