@@ -1392,28 +1392,31 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
         before = static_cast<E *>(a.grad) + (long long)r * a.grad_ld;
       }
       if (MODE == 1 && et >= nte - 32 && rank == 0) {  // the loss, by the last entry warp
-        Stat lst = no_stat();
-        if (rest) lst = combine_lanes<false, false>(lane % 2 < nwe ? listed[par][lane % 2] : no_stat(), 2, a.c);
         // With `rest` S is taken again in 64 bits from its two parts, relative to
         // the greater one's maximum: no gap between them is lost, and log S and
         // the log of the unlisted sum come from the same terms.
-        const bool parts = rest && su > 0.f, above = parts && lst.m > mu;
-        const double g = parts ? ((double)lst.m - mu) * a.inv_t_z : 0.0, x = exp_d(-fabs(g));
-        const double all = !parts ? (double)S : above ? lst.s + x * su : su + x * lst.s;
-        // every logarithm at once, a lane each
+        double all = S, gap = 0.0;  // what the listed maximum is above the unlisted one
+        float ref = m, tops = 1.f;  // what `all` is relative to, and how much of it is exact: a term of each part
+        if (rest && su > 0.f) {
+          const Stat lst = combine_lanes<false, false>(lane % 2 < nwe ? listed[par][lane % 2] : no_stat(), 2, a.c);
+          gap = ((double)lst.m - mu) * a.inv_t_z;
+          const double x = exp_d(-fabs(gap));
+          const bool above = lst.m > mu;
+          all = above ? lst.s + x * su : su + x * lst.s;
+          ref = above ? lst.m : mu;
+          tops = lst.s > 0.f ? 1.f + (float)x : 1.f;
+        }
+        // every logarithm at once, a lane each; lane 0 has its own at hand and the loss is its
         const double logs = log(lane == 0 ? all : lane == 1 ? (double)su : lane == 2 ? (double)S1 : rr);
         auto log_of = [&](int i) { return __shfl_sync(0xffffffffu, logs, i); };
         double l = 0;
         if (S == 0.f) {
           l = q_all > 0 ? INFINITY : 0.0;
         } else {
-          // the terms that are exact, one in each part
-          const float tops = parts && lst.s > 0.f ? 1.f + (float)x : 1.f;
-          const double log_s = log_of(0) + kEx2Low * (1.f - __fdividef(tops, (float)all));
+          const double log_s = logs + kEx2Low * (1.f - __fdividef(tops, (float)all));
           if (rr > 0.0)  // the student's rest is the unlisted sum over all
-            l = rr * (log_of(3) + (log_s - (log_of(1) + kEx2Low * (1.f - __fdividef(1.f, su)))) + (above ? g : 0.0));
-          const double ref = !parts ? m : above ? lst.m : mu;  // what log_s is relative to
-          for (int w = 0; w < nwe; ++w) l += sum_kl[w] + sum_q[par][w] * ((ref - list_top[w]) * a.inv_t_z);
+            l = rr * (log_of(3) + (log_s - (log_of(1) + kEx2Low * (1.f - __fdividef(1.f, su)))) + fmax(gap, 0.0));
+          for (int w = 0; w < nwe; ++w) l += sum_kl[w] + sum_q[par][w] * (((double)ref - list_top[w]) * a.inv_t_z);
           l += q_all * log_s;
         }
         l = a.a < 1.0 ? l * ((1.0 - a.a) * a.t * a.t) : 0.0;
