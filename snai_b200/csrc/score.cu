@@ -19,12 +19,13 @@
 // cut into slices over a cluster of CTAs when it is long.
 //
 // Measured on a B200 against its copy rate of 6553 GB/s (the bytes each
-// operator cannot do without over its time): 2048 x 131072 fp32 scores 1.04,
-// with 64 alternatives 0.71, distillation with the rest 0.87; 8192 x 16384
-// fp32 scores with 20 alternatives 0.58, gradient 0.83, distillation of 64
-// entries with labels 0.86; 8192 x 32000 bf16 scores 0.83, 2048 x 131072 bf16
-// gradient 0.79 (issue-bound: 11 lane instructions for two bytes of an element;
-// an eighth or a quarter of the exponentials on the FMA pipe made it slower).
+// operator cannot do without over its time): 2048 x 131072 fp32 scores 1.05,
+// with 64 alternatives 0.70, distillation with the rest 0.87; 8192 x 16384
+// fp32 scores with 20 alternatives 0.57, gradient 0.83, distillation of 64
+// entries with labels 0.86; 8192 x 32000 bf16 scores 0.81 and 2048 x 131072
+// bf16 gradient 0.78, where two bytes an element bring 9 and 15 lane
+// instructions: 70 and 56 % of the issue slots, 64 and 60 % of the pipe of
+// exponentials and conversions, none full, waiting for one another.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -1115,8 +1116,8 @@ __device__ __forceinline__ void cluster_meet() {
 //   grad_i = e_i alpha + gamma softmax(z)_i - what the list and the label take.
 // EXTRA: labels at T != 1, whose softmax needs exponentials of its own (1), or
 // at T = 2 or 4 the squares (2) or fourth powers (3) of those at hand
-// (8192 x 16384, 64 entries: 192 us against 215 with exponentials of their
-// own; 4096 x 32000 bf16: 133 against 169).  With `rest` the listed logits
+// (8192 x 16384, 64 entries: 191 us against 215 with exponentials of their
+// own; 4096 x 32000 bf16: 135 against 177).  With `rest` the listed logits
 // are taken out of the staged row (each by the thread that owns its word,
 // which finds it in a list of its own), so that the unlisted mass is a sum of
 // its own: 1 - the listed would lose a confident student's.
@@ -1128,7 +1129,7 @@ __device__ __forceinline__ void cluster_meet() {
 // out.  Pass B writes the terms that every element has; the entries' ids get
 // theirs from the entry threads one row later, behind the next row's barrier,
 // when all owners have written the base.  (Entries held by threads that also
-// take the row took 46 us where these took 34, at 1024 x 16384 with 64 entries
+// take the row took 46 us where these first took 34 (now 31), at 1024 x 16384 with 64 entries
 // and labels: their chain of dependent steps is as long as both passes.)  An
 // id listed more than once is handled by its first entry, in the order of the
 // list: no atomics.  The entries' weights and the loss are held in 64 bits: a
@@ -1662,12 +1663,17 @@ int row_words(const void *logits, int dtype, int vocab, long long ld) {
 
 // Streamed rows: a CTA a row, whatever its length.  When the rows leave SMs
 // short of CTAs a row is spread over a cluster of up to 8, down to slices of
-// 8 KB: until all CTAs are 7 halves of the SMs without alternatives (131072
-// fp32: 200 rows 21 us over pairs and 26 over one, 400 rows 40 and 35), 11
-// halves with few (these with three chunks in flight; 20: 200 rows 35 us over four, 59 over one; 250 rows 52 over
-// four and 42 over pairs; 512 rows of 16384 25 over pairs, 17 over one), and
-// twice with more, whose CTAs are twice as large and merge more (128: 100 rows
-// 34 us over pairs, 42 over one; 150 rows 56 and 46).
+// 8 KB, until all CTAs are so many halves of the SMs.
+//  7 without alternatives: 131072 fp32, 250 rows 25 us over pairs and 33 over
+//    one; past it 400 rows 39 over one and 35 over pairs, but 520 rows of 50001
+//    bf16 15 and 16.  (11 would give 150 rows of 131072 17 us over fours for 21
+//    over pairs, and 100 rows of 16384 6.1 over eights for 4.7 over fours.)
+// 11 with few: 20 of 131072, 200 rows 34 us over fours and 40 over pairs, 250
+//    rows 51 and 42, 400 rows 49 over pairs and 62 over one; 512 rows of 16384
+//    18.7 over pairs and 17.9 over one.
+//  4 with more, whose CTAs are twice as large and merge more: 128 of 131072,
+//    100 rows 34 us over pairs and 41 over one, 150 rows 56 and 46; 301 rows of
+//    50001 fp16 46 and 28.
 Plan plan_stream(const void *logits, int dtype, int rows, int vocab, long long ld, int top_k, int sms) {
   const int words = row_words(logits, dtype, vocab, ld);
   Plan p;
@@ -1759,9 +1765,10 @@ int by_dtype(int dtype, F &&f) {
   return f(__half());
 }
 
-// Chunks in flight a CTA.  One more each left a CTA less an SM: 301 rows of
-// 50001 fp16 with 128 alternatives 38 us for 27, 2048 x 131072 fp32 without
-// 167 for 157; only calls of few CTAs would gain (200 such rows 21 for 24).
+// Chunks in flight a CTA.  One more each leaves a CTA less an SM: 301 rows of
+// 50001 fp16 with 128 alternatives 40 us for 28, 2048 x 131072 fp32 without
+// 167 for 155; only calls of few CTAs would gain (200 such rows 20.5 for 23,
+// 400 of them 35 for 39).
 constexpr int kRing128 = 2, kRing256 = 3;
 
 template <typename E, int NT, int D>

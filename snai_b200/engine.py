@@ -446,7 +446,8 @@ def score_device(logits_dev, tokens_dev=None, temperature=1.0, top_k=0, want_ent
     """Log probabilities of tokens [rows] or [rows, n], entropies and the top_k
     alternatives of device logits [rows, vocab] (cortex_score), as a Score of
     device tensors.  Runs on `stream` (a handle), by default torch's current
-    stream of the logits' device."""
+    stream of the logits' device.  As all calls here it is no step of an
+    autograd graph: score_grad_device is its backward."""
     torch = _torch()
     code, rows, vocab, ld = _dev_rows(logits_dev)
     tok, n = _dev_tokens(tokens_dev, logits_dev, rows, torch.int32)
@@ -492,7 +493,7 @@ def distill_device(logits_dev, teacher_ids_dev, teacher_logits_dev, labels=None,
     """The distillation loss of device logits [rows, vocab] against a teacher's
     top logits [rows, k] (cortex_distill), and the gradient of
     sum(row_grad * loss), which may take the logits' place (grad_dev).
-    Returns (loss [rows], gradient or None)."""
+    Returns (loss [rows], gradient or None), tensors without an autograd graph."""
     torch = _torch()
     code, rows, vocab, ld = _dev_rows(logits_dev)
     if teacher_ids_dev.dim() != 2:
