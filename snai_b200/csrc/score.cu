@@ -1243,9 +1243,12 @@ __global__ void __launch_bounds__(NT + 32 * kMaxEntryWarps, NT == 128 ? 5 : 3) s
       alpha = -(float)q_all * k;
       if (ENT) alpha += gh * kLn2 * st.w * inv_s * k, beta = -gh * kLn2 * k;
     } else {
-      bool none = su == 0.f;  // of the student's unlisted probability is there in 64 bits (su is 0 or at least 1)
-      if (rest && f == 0.f) none = none || !((m - mu) * a.c + (__log2f(S) - __log2f(su)) < kNoRest);
-      rr = rest && !none ? fmax(0.0, 1.0 - q_all) : 0.0;
+      // Has the student any unlisted probability in 64 bits?  su is 0 or at least 1.
+      // All threads come to the same answer: rounded step by step, never contracted.
+      bool some = su > 0.f;
+      if (rest && f == 0.f)
+        some = some && __fadd_rn(__fmul_rn(m - mu, a.c), __fsub_rn(__log2f(S), __log2f(su))) < kNoRest;
+      rr = rest && some ? fmax(0.0, 1.0 - q_all) : 0.0;
       mass = (float)(q_all + rr);
       rest_k = rr > 0.0 ? (float)rr / su : 0.f;  // times an unlisted e_i: what the teacher's rest gives to i
       kt = sc * (float)((1.0 - a.a) * a.t);
