@@ -180,3 +180,40 @@ def test_rest_with_every_unlisted_id_masked(built):
         on[ids[r]] = True
         z[r, ~on] = -np.inf
     compare(z, "fp32", ids, vals, None, 1.0, 0.0, np.ones(len(z), dtype=np.float32))
+
+
+@pytest.mark.parametrize("left", [1e-6, 1e-8, 1e-9])
+def test_rest_that_a_list_nearly_fills(built, left):
+    """What the list leaves of 1 is a difference of 64-bit numbers, and so are
+    the gradients of the few unlisted ids: -r p_i / u for the greater part."""
+    V, k, R = 320, 300, 6
+    rng = np.random.default_rng(int(-np.log10(left)))
+    z = rng.normal(0, 1, (R, V)).astype(np.float32).astype(np.float64)
+    ids = np.stack([rng.choice(V, k, replace=False) for _ in range(R)]).astype(np.int32)
+    for r in range(R):  # unlisted ids of little probability: the rest's term is not lost beside their own
+        on = np.zeros(V, dtype=bool)
+        on[ids[r]] = True
+        z[r, ~on] -= 40.0
+    z = z.astype(np.float32).astype(np.float64)
+    q = rng.dirichlet(np.ones(k), R)
+    q[:, 0] = 0.7  # an exponential in the middle between two powers of 2, where it is hardest
+    q[:, 1:] *= 0.3 / q[:, 1:].sum(1, keepdims=True)
+    vals = np.log(q * (1 - left)).astype(np.float32)
+    for r in range(R):  # the float32 values' own sum is off by more than `left`: some take it up
+        for _ in range(60):
+            s = np.exp(vals[r].astype(np.float64)).sum()
+            j = int(np.argsort(-vals[r])[1 + _ % 30])
+            vals[r, j] = np.log(max(np.exp(float(vals[r, j])) + (1 - left - s), 1e-12))
+    rest = np.array([1 - np.exp(v.astype(np.float64)).sum() for v in vals])
+    keep = rest > left / 4
+    assert keep.sum() >= 2, rest
+    z, ids, vals, rest = z[keep], ids[keep], vals[keep], rest[keep]
+    _, grad = distill_device(on_gpu(z, "fp32"), torch.from_numpy(ids).to(DEV), torch.from_numpy(vals).to(DEV), rest=True)
+    got = grad.double().cpu().numpy()
+    for r in range(len(z)):
+        want = rest_row(z[r], ids[r], vals[r], -1, 1.0, 0.0)[1]
+        off = np.ones(V, dtype=bool)
+        off[ids[r]] = False
+        # r: 64-bit values, each to 1e-11 of itself, that make 1 in all; its share p_i / u: rel_err_bound
+        tol = (1e-11 / rest[r] + 2 * rel_err_bound(z[r], 1.0)) * np.abs(want[off])
+        assert (np.abs(got[r][off] - want[off]) <= tol).all(), (r, rest[r], got[r][off][:4], want[off][:4])
